@@ -16,6 +16,9 @@ LIB = os.path.join(HERE, "libdynam3d_hip.so")
 HOST_LIB = os.path.join(HERE, "libd3d_ffstate_host.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
+# no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results on this hardware now and then
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # (source, extra flags).  Geometry kernels are bit-exact against the oracle: no FMA contraction.
 HIP_SOURCES = [
     ("geometry_kernels.hip", ["-ffp-contract=off"]),
@@ -34,6 +37,8 @@ HIP_SOURCES = [
     ("mlp_kernels.hip", ["-ffp-contract=fast"]),
     ("segment_kernels.hip", ["-ffp-contract=off"]),
     ("ff_plan_kernels.hip", ["-ffp-contract=off"]),
+    ("fp8_quant_kernels.hip", ["-ffp-contract=off"] + NO_PACKED_F32),
+    ("fp8_gemm_kernels.hip", ["-ffp-contract=fast"] + NO_PACKED_F32),
 ]
 CPP_SOURCES = ["ff_state.cpp", "d3d_error.cpp", "phi3_decode.cpp", "mlp_forward.cpp"]
 HOST_CPP_SOURCES = ["ff_state.cpp", "d3d_error.cpp", "ff_plan_host.cpp"]      # the CPU-only bookkeeping library (no device entry points;

@@ -39,6 +39,13 @@ _lib.register("d3d_swiglu_f32", [vp, vp, i64, i32, vp])
 _lib.register("d3d_patchify_f32", [vp, vp, i32, i32, i32, i32, vp])
 _lib.register("d3d_vit_embed_ln_f32", [vp, vp, vp, vp, vp, vp, i32, i32, i32, f32, vp])
 _lib.register("d3d_assemble_prompt_f32", [vp, vp, vp, vp, vp, vp, vp, i32, i32, vp])
+# 8-bit linear layers (csrc/fp8_quant_kernels.hip, fp8_gemm_kernels.hip; called from fp8_ops)
+_lib.register("d3d_fp8_quantize", [vp, vp, vp, i32, i32, i64, i64, i64, i32, i32, vp])
+_lib.register("d3d_fp8_quantize_weight", [vp, vp, vp, i32, i32, i64, i64, i64, i32, i32, vp])
+_lib.register("d3d_fp8_dequantize", [vp, vp, vp, i32, i32, i64, i64, i64, i32, i32, i32, vp])
+_lib.register("d3d_fp8_rms_norm", [vp, vp, vp, vp, vp, vp, i32, i32, i64, i64, i64, i64, i64, f32, i32, i32, vp])
+_lib.register("d3d_fp8_gemm", [vp])
+_lib.register("d3d_fp8_gemm_workspace", [i32, i32, i32, i32])
 
 
 def _p(t: Optional[torch.Tensor]):

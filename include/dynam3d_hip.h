@@ -622,6 +622,42 @@ int32_t d3d_ffdev_flatten_zones(int32_t B, int32_t n_max, const int32_t* slot, c
 int32_t d3d_ffdev_live_ids(const d3d_ffdev_state* st, const int32_t* slot, int32_t B, int32_t* inst_ids, int32_t* n_inst,
                            int32_t* zone_ids, int32_t* n_zone, int32_t max_ids, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * 8-bit linear layers of the language model (csrc/fp8_quant_kernels.hip, fp8_gemm_kernels.hip).  The reference runs these layers in bf16
+ * (VLN-POL:119-131, 463); this is the same network with E4M3 operands: values in groups of 128 along K, one scale per group.
+ *   dtype: 0 bf16, 1 fp16, 2 float32.   scale_kind: 0 E8M0 bytes (s = 2^max(-126, ceil(log2(amax / 448)))), 1 float32
+ *   (s = max(amax / 448, 2^-126)); q = E4M3(x / s) rounded to nearest even, NaN where x is not finite (amax runs over the finite values).
+ *   Strides are in elements; rows of every matrix but the scales start on 16 bytes, K (D) is a multiple of 16.
+ * ---------------------------------------------------------------------------------------------- */
+/* x (rows, K) -> q (rows, K), scale (rows, ceil(K/128)) */
+int32_t d3d_fp8_quantize(const void* x, void* q, void* scale, int32_t rows, int32_t K, int64_t ldx, int64_t ldq, int64_t lds, int32_t dtype,
+                         int32_t scale_kind, void* stream);
+/* w (rows, K) -> q (rows, K), scale (ceil(rows/128), ceil(K/128)): one scale per 128 x 128 block */
+int32_t d3d_fp8_quantize_weight(const void* w, void* q, void* scale, int32_t rows, int32_t K, int64_t ldw, int64_t ldq, int64_t lds, int32_t dtype,
+                                int32_t scale_kind, void* stream);
+/* x = q * s, rounded once; group_rows = 1 (activations) or 128 (weights) */
+int32_t d3d_fp8_dequantize(const void* q, const void* scale, void* x, int32_t rows, int32_t K, int64_t ldq, int64_t lds, int64_t ldx, int32_t group_rows,
+                           int32_t dtype, int32_t scale_kind, void* stream);
+/* h = x [+ residual], rounded to the type of x and written to `sum` (residual == NULL: h = x, sum unused);
+ * (q, scale) = quantise(h * rsqrt(mean(h^2) + eps) * w), float32 inside; w float32, D <= 16384 */
+int32_t d3d_fp8_rms_norm(const void* x, const void* residual, const float* w, void* sum, void* q, void* scale, int32_t rows, int32_t D, int64_t ldx,
+                         int64_t ldr, int64_t ldsum, int64_t ldq, int64_t lds, float eps, int32_t dtype, int32_t scale_kind, void* stream);
+
+/* y = xq wq^T with the scales applied, float32 sums, + bias[n] + residual[m,n], rounded once to out_type (0 bf16, 1 fp16, 2 float32; bias and
+ * residual have that type; residual may be out).  swiglu: w = [gate (N/2 rows); up (N/2 rows)], y = up * silu(gate), (M, N/2), no bias or
+ * residual; out_type 3 = E4M3 + out_scale (M, ceil(N/2/128)) of the same scale_kind.  Both scales are of scale_kind; a product of two
+ * scales must be a finite float32.  `workspace`: d3d_fp8_gemm_workspace() bytes of device memory on 16 bytes, used until the call's work
+ * on `stream` has ended (0: none needed). */
+typedef struct d3d_fp8_gemm_args {
+    const void *x, *sx, *w, *sw, *bias, *residual;
+    void *out, *out_scale, *workspace;
+    int64_t workspace_bytes, ldx, ldsx, ldw, ldsw, ldr, ldo, ldos;
+    int32_t M, N, K, scale_kind, out_type, swiglu;
+    void* stream;
+} d3d_fp8_gemm_args;
+int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu);
+int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* a);
+
 #ifdef __cplusplus
 }
 #endif

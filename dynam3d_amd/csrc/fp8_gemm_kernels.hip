@@ -56,6 +56,12 @@ __device__ __forceinline__ void dma_piece_at(const uint8_t* addr, uint32_t dst) 
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(addr), "s"(d) : "memory");
 }
+__device__ __forceinline__ void dma_piece_once(uint32_t voff, const uint8_t* base, uint32_t dst) {      // data read once: not kept in the caches
+    const uint32_t d = __builtin_amdgcn_readfirstlane(dst);
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 
 __device__ __forceinline__ v8i frag(const uint8_t* lo, const uint8_t* hi) {
@@ -395,7 +401,173 @@ k_fp8_gemm_tile(const GemmArgs a) {
     }
 }
 
-// ---- split K: the slices' float32 sums, added in slice order, and the epilogue ---------------------------------------------------------------
+// ================================================================================================================================
+// Few rows (M <= 16 MT): the weights stream once.
+//   * A workgroup owns R neighbouring rows of w (SwiGLU: R gate rows and the R up rows beside them), R chosen so that the grid is one or a few whole
+//     workgroups per CU; its waves take the K blocks in turn (block b to wave b mod waves: side by side they read neighbouring 128 B of the same
+//     rows).  A wave requests up to nb blocks before it waits, so that a CU has ~100 KB in flight: what bounds it is memory, then the launch.
+//   * The blocks go to the wave's own corner of LDS by DMA, 8 rows x 128 B per instruction, not cached (nt): that pattern reads 28 MB of cold weights
+//     in 6.1 us, fragments loaded straight into registers (16 rows x 64 B) in 7.2 and more registers.  No barrier: each wave reads what it loaded.
+//   * x, at most MT x 16 rows out of L2, takes the same way, once per workgroup; the scales of a batch of blocks are one load each for x and w, a lane
+//     per scale, handed round with cross-lane reads (a byte load per use cost 1 us of 10: the address pipe takes 16 cycles per instruction).
+//   * 16-bit results take the 8-bit instruction; float32 ones, and up to 32 rows those that are quantised again, the EXACT product (see the top).
+//   * The waves' sums meet in LDS and are added in wave order; one thread then has 4 neighbouring columns of a row.
+// ================================================================================================================================
+template <int KIND, bool SWI, bool EXACT, int MT, int NJ, int U, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64)
+k_fp8_gemm_rows(const GemmArgs a, int R /* <= 16 NJ, a multiple of 4 */, int nb /* blocks in flight per wave, <= U */) {
+    constexpr int NT = SWI ? 2 : 1, NW = NJ * NT, T = MT * NW, ESZ = KIND == 0 ? 1 : 4, SLOT = (NW + MT) * 2048;
+    static_assert(U * MT <= 4, "one lane per x scale of a batch");
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];     // [waves][nb][NT][NJ][16 rows of w][128 B], [MT][16 rows of x][128 B]; then [waves][T][64] sums
+    v4f* red = reinterpret_cast<v4f*>(smem);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = (int)blockDim.x >> 6;
+    const int fi = lane & 15, fg = lane >> 4, lr = lane >> 3;
+    const int ncols = SWI ? a.I : a.N, n0 = (int)blockIdx.x * R, rows = min(R, ncols - n0);
+    const int chunk = (lane & 7) ^ lr;                                 // source chunk of this lane in every piece of 8 rows
+    const uint32_t wo = (uint32_t)(lr * a.ldw) + chunk * 16, xo = (uint32_t)(lr * a.ldx) + chunk * 16;
+    // lane -> x scale (block u, row): u * MT * 16 + row; lane -> w scale: u * 4 + half * 2 + (0: the block of 128 of the first row, 1: of the last)
+    const uint8_t* sxl = (const uint8_t*)a.sx + (int64_t)min(lane % (MT * 16), a.M - 1) * a.ldsx * ESZ;
+    const uint8_t* swl = (const uint8_t*)a.sw + (int64_t)(((SWI && (lane & 2) ? a.I : 0) + n0 + (lane & 1 ? rows - 1 : 0)) >> 7) * a.ldsw * ESZ;
+    // lane of the w scale of its operand row (E8M0 in the instruction) or of its 4 result columns (they lie in one block)
+    int swi_lane[NW];
+#pragma unroll
+    for (int t = 0; t < NW; ++t) {
+        const int half = t / NJ, first = (half ? a.I : 0) + n0, r = first + min((t % NJ) * 16 + (!EXACT && KIND == 0 ? fi : fg * 4), rows - 1);
+        swi_lane[t] = half * 2 + ((r >> 7) != (first >> 7) ? 1 : 0);
+    }
+    v4f acc[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+
+    auto scale_at = [&](const uint8_t* p, int kb) { return KIND == 0 ? (uint32_t)p[kb] : ((const uint32_t*)p)[kb]; };
+    auto frag_at = [&](const uint8_t* p, int h) { return *reinterpret_cast<const v4i*>(p + fi * FP8_G + (((fg + 4 * h) ^ (fi & 7)) << 4)); };
+    const uint8_t* mine = smem + (uint32_t)wave * nb * SLOT;
+    const uint32_t dst0 = lds_addr(smem) + (uint32_t)wave * nb * SLOT;
+    for (int b0 = wave; b0 < a.KB; b0 += nw * nb) {
+        const uint32_t vx = scale_at(sxl, min(b0 + lane / (MT * 16) * nw, a.KB - 1)), vw = scale_at(swl, min(b0 + (lane >> 2) * nw, a.KB - 1));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // the reads of the blocks before have left LDS
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = b0 + u * nw;
+            if (u >= nb || b >= a.KB) continue;
+            const bool in = b * FP8_G + chunk * 16 < a.K, ragged = b * FP8_G + FP8_G > a.K;
+            const uint32_t dst = dst0 + (uint32_t)(u * SLOT);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int q = 0; q < NJ * 2; ++q) {
+                    if (q * 8 >= rows) break;                          // (the same for the whole workgroup)
+                    const uint8_t* base = a.w + ((int64_t)(n0 + q * 8 + (t ? a.I : 0)) * a.ldw + (int64_t)b * FP8_G);
+                    if (q * 8 + lr < rows) {                           // rows of the neighbour are not read; their part of LDS feeds results that nobody stores
+                        if (ragged) dma_piece_at(in ? base + wo : (const uint8_t*)&g_zero16, dst + (t * NJ * 2 + q) * 1024);
+                        else dma_piece_once(wo, base, dst + (t * NJ * 2 + q) * 1024);
+                    }
+                }
+#pragma unroll
+            for (int q = 0; q < MT * 2; ++q) {
+                if (q * 8 >= a.M) break;
+                const uint8_t* base = a.x + ((int64_t)q * 8 * a.ldx + (int64_t)b * FP8_G);
+                if (q * 8 + lr < a.M) {
+                    if (ragged) dma_piece_at(in ? base + xo : (const uint8_t*)&g_zero16, dst + (NW * 2 + q) * 1024);
+                    else dma_piece(xo, base, dst + (NW * 2 + q) * 1024);
+                }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= nb || b0 + u * nw >= a.KB) continue;
+            const uint8_t* slot = mine + u * SLOT;
+            v4i x[MT][2];
+            uint32_t sx[MT], sw[NW];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                x[i][0] = frag_at(slot + (NW + i) * 2048, 0);
+                x[i][1] = frag_at(slot + (NW + i) * 2048, 1);
+                sx[i] = __shfl(vx, (u * MT + i) * 16 + fi, 64);
+            }
+#pragma unroll
+            for (int t = 0; t < NW; ++t) sw[t] = __shfl(vw, u * 4 + swi_lane[t], 64);
+            if constexpr (!EXACT) {
+#pragma unroll
+                for (int t = 0; t < NW; ++t) {
+                    const v8i w = __builtin_shufflevector(frag_at(slot + t * 2048, 0), frag_at(slot + t * 2048, 1), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const v8i xv = __builtin_shufflevector(x[i][0], x[i][1], 0, 1, 2, 3, 4, 5, 6, 7);
+                        if constexpr (KIND == 0) {
+                            acc[i * NW + t] = mma_scaled(w, xv, acc[i * NW + t], sw[t], sx[i]);
+                        } else {
+                            const v4f d = mma_plain(w, xv, v4f{0.f, 0.f, 0.f, 0.f});
+                            const float s = __uint_as_float(sx[i]) * __uint_as_float(sw[t]);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[i * NW + t][r] = __builtin_fmaf(d[r], s, acc[i * NW + t][r]);
+                        }
+                    }
+                }
+            } else {
+                bf8 xh[MT][4];
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) xh[i][g] = to_bf16(x[i][g >> 1][(g & 1) * 2], x[i][g >> 1][(g & 1) * 2 + 1]);
+#pragma unroll
+                for (int t = 0; t < NW; ++t) {
+                    v4f d[MT];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) d[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const v4i w = frag_at(slot + t * 2048, h);
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const bf8 wh = to_bf16(w[g * 2], w[g * 2 + 1]);
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wh, xh[i][h * 2 + g], d[i], 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const float s = scale_value(sx[i], KIND) * scale_value(sw[t], KIND);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i * NW + t][r] = __builtin_fmaf(d[i][r], s, acc[i * NW + t][r]);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();                                                   // every wave has read its blocks: LDS becomes the sums
+#pragma unroll
+    for (int t = 0; t < T; ++t) red[(wave * T + t) * 64 + lane] = acc[t];
+    __syncthreads();
+    for (int e = tid; e < MT * NJ * 64; e += (int)blockDim.x) {        // (m tile, column tile, lane): 4 columns of one row
+        const int i = e / (NJ * 64), j = (e >> 6) % NJ, l = e & 63, m = i * 16 + (l & 15), c = j * 16 + (l >> 4) * 4, n = n0 + c;
+        if (m >= a.M || c >= rows) continue;
+        float v[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const v4f* p = red + (i * NW + t * NJ + j) * 64 + l;
+            v4f s = p[0];
+#pragma unroll
+            for (int q = 1; q < WAVES; ++q)
+                if (q < nw) s += p[q * T * 64];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[t][r] = s[r];
+        }
+        if constexpr (SWI) {
+            if (a.out_type == 3) {                                     // k_fp8_gemm_finish needs 128 columns for a scale
+                *reinterpret_cast<v4f*>(a.ws + (int64_t)m * a.ldws + n) = v4f{v[0][0], v[0][1], v[0][2], v[0][3]};
+                *reinterpret_cast<v4f*>(a.ws + (int64_t)m * a.ldws + a.ldws / 2 + n) = v4f{v[1][0], v[1][1], v[1][2], v[1][3]};
+                continue;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[0][r] = v[1][r] * silu(v[0][r]);
+        }
+        finish4(a, v[0], m, n, n0 + rows);
+    }
+}
+
+// ---- split K: the slices float32 sums, added in slice order, and the epilogue ---------------------------------------------------------------
 // 8 columns per thread; 16 threads are one group of 128 columns of the quantised result.
 __global__ void __launch_bounds__(256)
 k_fp8_gemm_finish(const GemmArgs a, int swi, int c8 /* threads per row: a multiple of 16 */, int kind) {
@@ -448,13 +620,24 @@ k_fp8_gemm_finish(const GemmArgs a, int swi, int c8 /* threads per row: a multip
 constexpr int CUS = 256;
 
 struct Plan {
+    int rows;                                                          // 16-row tiles of k_fp8_gemm_rows; 0: tile kernel
     int bm, bn, tiles_m, tiles_n, splits;
     int64_t ldws, ws_bytes;
 };
 
-Plan plan_of(int M, int N, int K, bool swi) {
+Plan plan_of(int M, int N, int K, bool swi, int out_type) {
     Plan p{};
     const int KB = (K + FP8_G - 1) / FP8_G, ncols = swi ? N / 2 : N;
+    p.ldws = swi ? 2 * ((ncols + 7) / 8 * 8) : (ncols + 7) / 8 * 8;
+    // Few rows: the weights stream once (device time at K = 3072, N = 9216, us, against the tile kernel: M = 17 9.4 : 15.1, 32 10.4 : 16.0, 64 13.3 : 18.0;
+    // K = 8192, N = 3072: 32 12.3 : 18.7, 64 16.5 : 20.1).  Behind 32 rows x is most of what a workgroup of a wide product reads: N = 32064 at 64 rows
+    // 40.1 : 34.0.
+    if (M <= 32 || (M <= 64 && ncols <= 64 * CUS)) {
+        p.rows = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+        p.splits = 1;
+        p.ws_bytes = out_type == 3 ? (int64_t)M * p.ldws * 4 : 0;
+        return p;
+    }
     p.bm = swi ? 64 : 128;
     p.bn = 128;                                                        // columns of the result per tile (SwiGLU: 256 rows of w)
     p.tiles_m = (M + p.bm - 1) / p.bm;
@@ -462,7 +645,6 @@ Plan plan_of(int M, int N, int K, bool swi) {
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     // fewer tiles than one round of two workgroups per CU: cut K so that a round is filled, at least 4 K tiles per slice
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * CUS / tiles, KB / 4));
-    p.ldws = swi ? 2 * ((ncols + 7) / 8 * 8) : (ncols + 7) / 8 * 8;
     p.ws_bytes = p.splits > 1 ? (int64_t)p.splits * M * p.ldws * 4 : 0;
     return p;
 }
@@ -495,13 +677,51 @@ int32_t launch_tile(const GemmArgs& a, hipStream_t s) {
     D3D_LAUNCH_CHECK();
 }
 
+template <int KIND, bool SWI, bool EXACT, int MT, int NJ>
+int32_t launch_rows_of(const GemmArgs& a, int R, hipStream_t s) {
+    constexpr int NW = NJ * (SWI ? 2 : 1), T = MT * NW, U = 4 / MT, WAVES = SWI || MT == 4 ? 8 : 16, SLOT = (NW + MT) * 2048, LDS = 160 * 1024;
+    const int grid = ((SWI ? a.I : a.N) + R - 1) / R;
+    const int per = (a.KB + WAVES - 1) / WAVES, nw = (a.KB + per - 1) / per;                    // K blocks of a wave; the waves that takes
+    // more workgroups than CUs: two of them per CU, so that one loads while the other adds up (16384 x 3072 at 8 rows: 12.2 us; one, with twice
+    // the blocks in flight: 14.2)
+    const int nb = std::min({U, per, std::max(1, (grid > CUS ? LDS / 2 : LDS) / (nw * SLOT))});
+    const size_t sh = (size_t)nw * std::max(nb * SLOT, T * 1024);
+    static_assert(WAVES * (SLOT > T * 1024 ? SLOT : T * 1024) <= LDS, "one block per wave fits");
+    static std::atomic<uint64_t> done{0};
+    const int32_t rc = allow_lds(reinterpret_cast<const void*>(&k_fp8_gemm_rows<KIND, SWI, EXACT, MT, NJ, U, WAVES>), LDS, done);
+    if (rc != D3D_OK) return rc;
+    hipLaunchKernelGGL((k_fp8_gemm_rows<KIND, SWI, EXACT, MT, NJ, U, WAVES>), dim3((uint32_t)grid), dim3(nw * 64), sh, s, a, R, nb);
+    D3D_LAUNCH_CHECK();
+}
+template <int KIND, bool SWI, bool EXACT, int MT>
+int32_t launch_rows(const GemmArgs& a, hipStream_t s) {
+    // R: one workgroup per CU up to 48 rows (SwiGLU: 16), else a whole number of them of up to 32
+    constexpr int MOST = SWI ? 16 : 48, MANY = SWI ? 16 : 32;
+    const int ncols = SWI ? a.I : a.N, per_cu = ncols <= CUS * MOST ? 1 : (ncols + CUS * MANY - 1) / (CUS * MANY);
+    const int R = std::max(8, ((ncols + CUS * per_cu - 1) / (CUS * per_cu) + 3) / 4 * 4);
+    if constexpr (MOST > 16) {
+        if (R > 32) return launch_rows_of<KIND, SWI, EXACT, MT, 3>(a, R, s);
+        if (R > 16) return launch_rows_of<KIND, SWI, EXACT, MT, 2>(a, R, s);
+    }
+    return launch_rows_of<KIND, SWI, EXACT, MT, 1>(a, R, s);
+}
+template <int KIND, bool SWI>
+int32_t launch(const GemmArgs& a, int rows, hipStream_t s) {
+    // a result that is quantised again is EXACT too while that is free (8 rows of 8192 x 3072: 15.7 us; at 64 rows 32.4 against 25.6)
+    const bool exact = a.out_type == 2 || (a.out_type == 3 && rows <= 2);
+    if (rows == 1) return exact ? launch_rows<KIND, SWI, true, 1>(a, s) : launch_rows<KIND, SWI, false, 1>(a, s);
+    if (rows == 2) return exact ? launch_rows<KIND, SWI, true, 2>(a, s) : launch_rows<KIND, SWI, false, 2>(a, s);
+    if (rows == 4) return exact ? launch_rows<KIND, SWI, true, 4>(a, s) : launch_rows<KIND, SWI, false, 4>(a, s);
+    return a.out_type == 2 ? launch_tile<KIND, SWI, true>(a, s) : launch_tile<KIND, SWI, false>(a, s);
+}
+
 }  // namespace
 
 extern "C" {
 
-int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu) {
+int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return plan_of(M, N, K, swiglu != 0).ws_bytes;
+    return plan_of(M, N, K, swiglu != 0, out_type).ws_bytes;
 }
 
 int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
@@ -520,8 +740,8 @@ int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
     if (g->ldx >= (int64_t)1 << 24 || g->ldw >= (int64_t)1 << 24) return bad("d3d_fp8_gemm: rows further than 16 MiB apart");
     if (g->ldsx < 0 || g->ldsw < 0 || g->ldsx >= 1 << 20 || (int64_t)(g->N / FP8_G + 1) * g->ldsw >= 1 << 29) return bad("d3d_fp8_gemm: scale rows too far apart");
     if (swi && (int64_t)g->N * g->ldw >= (int64_t)1 << 32) return bad("d3d_fp8_gemm: SwiGLU weights of 4 GiB and more");
-    const Plan p = plan_of(g->M, g->N, g->K, swi);
-    if ((int64_t)p.tiles_m * p.tiles_n * p.splits >= (int64_t)1 << 31) return bad("d3d_fp8_gemm: too many tiles for one launch");
+    const Plan p = plan_of(g->M, g->N, g->K, swi, g->out_type);
+    if (!p.rows && (int64_t)p.tiles_m * p.tiles_n * p.splits >= (int64_t)1 << 31) return bad("d3d_fp8_gemm: too many tiles for one launch");
     if (p.ws_bytes > g->workspace_bytes || (p.ws_bytes && (!g->workspace || ((uintptr_t)g->workspace & 15))))
         return bad("d3d_fp8_gemm: workspace smaller than d3d_fp8_gemm_workspace() or not on 16 bytes");
     GemmArgs a{};
@@ -535,12 +755,9 @@ int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
     a.vec = g->out_type == 3 || (((uintptr_t)g->out % eb) == 0 && (g->ldo * es) % eb == 0 &&
                                  (!g->residual || (((uintptr_t)g->residual % eb) == 0 && (g->ldr * es) % eb == 0)));
     hipStream_t s = (hipStream_t)g->stream;
-    const int32_t rc = g->out_type == 2
-                           ? (swi ? (g->scale_kind == 0 ? launch_tile<0, true, true>(a, s) : launch_tile<1, true, true>(a, s))
-                                  : (g->scale_kind == 0 ? launch_tile<0, false, true>(a, s) : launch_tile<1, false, true>(a, s)))
-                           : (swi ? (g->scale_kind == 0 ? launch_tile<0, true, false>(a, s) : launch_tile<1, true, false>(a, s))
-                                  : (g->scale_kind == 0 ? launch_tile<0, false, false>(a, s) : launch_tile<1, false, false>(a, s)));
-    if (rc != D3D_OK || p.splits == 1) return rc;
+    const int32_t rc = swi ? (g->scale_kind == 0 ? launch<0, true>(a, p.rows, s) : launch<1, true>(a, p.rows, s))
+                           : (g->scale_kind == 0 ? launch<0, false>(a, p.rows, s) : launch<1, false>(a, p.rows, s));
+    if (rc != D3D_OK || !p.ws_bytes) return rc;
     const int c8 = (ncols + 127) / 128 * 16;
     const int64_t nb = ((int64_t)a.M * c8 + 255) / 256;
     hipLaunchKernelGGL(k_fp8_gemm_finish, dim3((uint32_t)nb), dim3(256), 0, s, a, swi ? 1 : 0, c8, g->scale_kind);

@@ -54,6 +54,13 @@ class Fp8:
             raise ValueError(f"Fp8: scale {tuple(scale.shape)} on {scale.device} does not fit data {tuple(data.shape)} on {data.device} with one scale per {rows} rows")
         self.data, self.scale, self.rows = data, scale, rows
 
+    @staticmethod
+    def _of(data, scale, rows=1):
+        """(unchecked: for results made here)"""
+        r = object.__new__(Fp8)
+        r.data, r.scale, r.rows = data, scale, rows
+        return r
+
     @property
     def shape(self):
         return self.data.shape
@@ -107,7 +114,7 @@ def _same_device(name, first, *others):
             raise ValueError(f"fp8_ops.{name}: operands on {first.device} and {t.device}")
 
 
-# ---- the expressions in PyTorch (CPU tensors) ----------------------------------------------------------------------------------------------
+# ---- the expressions in PyTorch (CPU tensors; no gradient, like the kernels) ----------------------------------------------------------------------------------------------
 def _cpu_scale(amax, scale_dtype):
     if scale_dtype == torch.float32:
         return torch.clamp(amax / E4M3_MAX, min=_LEAST)
@@ -121,6 +128,7 @@ def _cpu_groups(x):
     return torch.nn.functional.pad(x, (0, pad)).view(x.shape[0], (x.shape[1] + pad) // GROUP, GROUP)
 
 
+@torch.no_grad()
 def _cpu_quantize(x, scale_dtype, rows):
     xg = _cpu_groups(x.float())
     a = torch.where(xg.isfinite(), xg.abs(), torch.zeros_like(xg)).amax(-1)
@@ -132,6 +140,7 @@ def _cpu_quantize(x, scale_dtype, rows):
     return Fp8(t.flatten(1)[:, :x.shape[1]].to(E4M3).contiguous(), s.to(scale_dtype), rows)
 
 
+@torch.no_grad()
 def _cpu_values(q: Fp8):
     s = q.scale.float().repeat_interleave(q.rows, 0)[:q.data.shape[0]]
     return (_cpu_groups(q.data.float()) * s[:, :, None]).flatten(1)[:, :q.data.shape[1]]
@@ -152,22 +161,19 @@ def _quantize(name, x, scale_dtype, rows):
     lib = _lib.load()
     _lib.check((lib.d3d_fp8_quantize if rows == 1 else lib.d3d_fp8_quantize_weight)(x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0), k, s.shape[1],
                                                                                     _DT[x.dtype], _KIND[scale_dtype], _stream()))
-    return Fp8(q, s, rows)
+    return Fp8._of(q, s, rows)
 
 
-@torch.no_grad()
 def quantize(x: torch.Tensor, scale_dtype: torch.dtype = E8M0) -> Fp8:
     """x (rows, K) bf16 / fp16 / float32, K a multiple of 16 -> E4M3 with one scale per row and group of 128 columns."""
     return _quantize("quantize", x, scale_dtype, 1)
 
 
-@torch.no_grad()
 def quantize_weight(w: torch.Tensor, scale_dtype: torch.dtype = E8M0) -> Fp8:
     """w (out, in) -> E4M3 with one scale per 128 x 128 block: what `linear` and `linear_swiglu` take, made once per weight."""
     return _quantize("quantize_weight", w, scale_dtype, GROUP)
 
 
-@torch.no_grad()
 def dequantize(q: Fp8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values q.data * q.scale, rounded once to `dtype` (exact in bf16 for power-of-two scales)."""
     if dtype not in _DT or dtype == E4M3:
@@ -187,7 +193,6 @@ def dequantize(q: Fp8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return x
 
 
-@torch.no_grad()
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None, scale_dtype: torch.dtype = E8M0):
     """quantise(h / sqrt(mean(h^2) + eps) * w) for the rows of h = x, or of h = x + residual rounded to x's type; float32 inside, one rounding,
     to E4M3.  x (rows, D), D a multiple of 16 up to 16384; w (D) float32.  -> Fp8, with a residual (Fp8, h): h is the next residual stream."""
@@ -199,9 +204,10 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float, residual: Optional[to
         raise TypeError(f"fp8_ops.rms_norm: residual {tuple(residual.shape)} {residual.dtype} beside x {tuple(x.shape)} {x.dtype}")
     _same_device("rms_norm", x, w, residual)
     if not x.is_cuda:
-        h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
-        hf = h.float()
-        q = _cpu_quantize(hf / torch.sqrt((hf * hf).mean(-1, keepdim=True) + eps) * w, scale_dtype, 1)
+        with torch.no_grad():
+            h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+            hf = h.float()
+            q = _cpu_quantize(hf / torch.sqrt((hf * hf).mean(-1, keepdim=True) + eps) * w, scale_dtype, 1)
         return q if residual is None else (q, h)
     if d > 16384:
         raise ValueError(f"fp8_ops.rms_norm: rows of {d} columns: at most 16384")
@@ -219,15 +225,16 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float, residual: Optional[to
         hp, rp, ldr = h.data_ptr(), residual.data_ptr(), residual.stride(0)
     _lib.check(_lib.load().d3d_fp8_rms_norm(x.data_ptr(), rp, w.data_ptr(), hp, q.data_ptr(), s.data_ptr(), m, d, x.stride(0), ldr, d, d, s.shape[1],
                                             float(eps), _DT[x.dtype], _KIND[scale_dtype], _stream()))
-    return Fp8(q, s) if residual is None else (Fp8(q, s), h)
+    q = Fp8._of(q, s)
+    return q if residual is None else (q, h)
 
 
 # ---- products --------------------------------------------------------------------------------------------------------------------------------
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(m, n, k, swiglu):
+def _workspace_bytes(m, n, k, swiglu, out_type):
     fn = _lib.load().d3d_fp8_gemm_workspace
     fn.restype = C.c_int64
-    return fn(m, n, k, swiglu)
+    return fn(m, n, k, swiglu, out_type)
 
 
 def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):
@@ -242,7 +249,7 @@ def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):
         ldos = (cols + GROUP - 1) // GROUP
         out_scale = torch.empty((m, ldos), dtype=sx.dtype, device=dev)
         osp = out_scale.data_ptr()
-    nbytes = _workspace_bytes(m, n, k, swiglu)
+    nbytes = _workspace_bytes(m, n, k, swiglu, _DT[out_dtype])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None      # (stream-ordered: torch's allocator, or the capturing graph's pool)
     bp, rp, ldr = None, None, 0
     if bias is not None:
@@ -254,7 +261,7 @@ def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):
     a = _GemmArgs(xd.data_ptr(), sx.data_ptr(), wd.data_ptr(), sw.data_ptr(), bp, rp, out.data_ptr(), osp, ws.data_ptr() if nbytes else None, nbytes,
                   xd.stride(0), sx.stride(0), wd.stride(0), sw.stride(0), ldr, cols, ldos, m, n, k, _KIND[sx.dtype], _DT[out_dtype], swiglu, _stream())
     _lib.check(_lib.load().d3d_fp8_gemm(C.byref(a)))
-    return out if out_scale is None else Fp8(out, out_scale)
+    return out if out_scale is None else Fp8._of(out, out_scale)
 
 
 def _check_operands(name, x, w):
@@ -268,7 +275,6 @@ def _check_operands(name, x, w):
         raise ValueError(f"fp8_ops.{name}: operands on {x.device} and {w.device}")
 
 
-@torch.no_grad()
 def linear(x: Fp8, w: Fp8, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x w^T [+ bias] [+ residual]: x (M, K), w (N, K), float32 sums, rounded once to `out_dtype` (bf16, fp16, float32 -- the type of bias (N,) and
@@ -283,17 +289,17 @@ def linear(x: Fp8, w: Fp8, bias: Optional[torch.Tensor] = None, residual: Option
         raise TypeError(f"fp8_ops.linear: residual ({m}, {n}) {out_dtype}, not {tuple(residual.shape)} {residual.dtype}")
     _same_device("linear", x.data, bias, residual)
     if not x.data.is_cuda:
-        y = _cpu_values(x) @ _cpu_values(w).t()
-        for e in (bias, residual):
-            y = y if e is None else y + e.float()
-        return y.to(out_dtype)
+        with torch.no_grad():
+            y = _cpu_values(x) @ _cpu_values(w).t()
+            for e in (bias, residual):
+                y = y if e is None else y + e.float()
+            return y.to(out_dtype)
     if x.data.get_device() != _current_device():
         with torch.cuda.device(x.device):
             return _gemm("linear", x, w, bias, residual, out_dtype, 0)
     return _gemm("linear", x, w, bias, residual, out_dtype, 0)
 
 
-@torch.no_grad()
 def linear_swiglu(x: Fp8, w: Fp8, out_dtype: torch.dtype = torch.bfloat16):
     """up * silu(gate) of x w^T, w = [gate (I rows); up (I rows)] as HF's `gate_up_proj` has them, I a multiple of 16; float32 up to the ONE rounding:
     to bf16 / fp16 / float32, or with out_dtype=torch.float8_e4m3fn to an `Fp8` (scales of the operands' type) for the product that follows."""

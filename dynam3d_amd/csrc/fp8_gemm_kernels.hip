@@ -15,6 +15,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
+#include <utility>
 
 #include "../../include/dynam3d_hip.h"
 #include "d3d_common.h"
@@ -402,6 +404,272 @@ k_fp8_gemm_tile(const GemmArgs a) {
 }
 
 // ================================================================================================================================
+// Large products, E8M0 scales, results of 8 or 16 bits: 256 x 256 x 128 per workgroup of FOUR waves, 128 x 128 each, one wave per SIMD.
+//   * 64 products of 16x16x128 per wave and K tile on 256 accumulators, out of 16 fragments that stay in registers; a fragment is replaced by the next
+//     K tile's as its last product issues, 12 products (400 cycles) and more ahead of its use.  LDS is read 128 KiB per K tile; with 128 x 64 per
+//     wave (eight waves) it was 192, the two waves of a SIMD met at the barriers, and the matrix pipe was busy 58 % of the time.
+//   * Two barriers per K tile: behind the first every wave has read tile p and its buffer takes the DMA of tile p + 2; behind the second tile p + 1
+//     has landed.  A load so has 1.3 tiles (2700 cycles and more) to arrive.
+//   * 16x16x128 products: the matrix pipe alone runs 4.3 PFLOP/s on them and 3.6 - 3.9 on 32x32x64 (power), measured on random data.
+//   * Rows are permuted inside blocks of 64: row 4 f + c of a block is row f of tile c, for x and w alike.  A lane then holds 16 NEIGHBOURING columns of a row
+//     (it stores them with no trip through LDS), and the scales of its rows in four tiles are neighbours: they come by DMA too, a dword per row, are
+//     read as one 16-byte piece, and packed into a register of which the instruction picks the byte.
+// DT: 0 bf16, 1 fp16, 3 E4M3 + scale (SwiGLU).  Rows of out and residual allow 16-byte accesses, columns come in eights (the host's choice of this kernel).
+// ================================================================================================================================
+// 1 KiB (16 bytes per lane from base + off), or one byte per lane into a dword, to LDS dst + IMM; base and dst in scalar registers.  (m0 is not kept: nothing else
+// in the kernel below uses it.)
+template <int IMM>
+__device__ __forceinline__ void dma_to(uint32_t off, const uint8_t* base, uint32_t dst) {
+    asm volatile("s_add_u32 m0, %1, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(off), "s"(dst), "s"(base), "n"(IMM) : "memory", "scc");
+}
+template <int IMM>
+__device__ __forceinline__ void dma_byte_to(uint32_t off, const uint8_t* base, uint32_t dst) {
+    asm volatile("s_add_u32 m0, %1, %3\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, %2" ::"v"(off), "s"(dst), "s"(base), "n"(IMM) : "memory", "scc");
+}
+
+template <class F, int... I>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) { each(f, std::make_integer_sequence<int, N>{}); }
+
+template <bool SWI, int DT>
+__global__ void __launch_bounds__(256, 1)
+k_fp8_gemm_big(const GemmArgs a) {
+    constexpr int BM = 256, BN = 256, BUF = (BM + BN) * FP8_G, OUT_N = SWI ? BN / 2 : BN;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];     // [2][x 256 x 128 | w 256 x 128], scales [2][4 waves][4][64] dwords
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1, fi = lane & 15, fg = lane >> 4, lr = lane >> 3;
+    const int ncols = SWI ? a.I : a.N, nk = a.KB;
+    const int nwg = a.tiles_m * a.tiles_n;
+    int wg = blockIdx.x;
+    {
+        const int xcd = wg & 7, q = nwg >> 3, r = nwg & 7;
+        wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (wg >> 3);
+    }
+    constexpr int GM = 4;                                              // 4 row tiles share the w tiles of an XCD: 4 + 8 operand panels for its 32 workgroups
+    const int g0 = wg / (GM * a.tiles_n) * GM, gs = min(GM, a.tiles_m - g0), ti = wg % (GM * a.tiles_n);
+    const int row0 = __builtin_amdgcn_readfirstlane((g0 + ti % gs) * BM), col0 = __builtin_amdgcn_readfirstlane(ti / gs * OUT_N);
+
+    // DMA: piece q of a wave is LDS rows (wave + 4 q) * 8 .. + 7 of an operand tile; offsets from the tile's origin, rows behind the end read the last
+    // one again (their results are not stored).  Chunk swizzle ^ (LDS row & 7).
+    const int chunk = (lane & 7) ^ lr;
+    const uint8_t* xbase = a.x + (int64_t)row0 * a.ldx;
+    const uint8_t* wbase = a.w + (SWI ? 0 : (int64_t)col0 * a.ldw);
+    uint32_t xo[8], wo[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const int r = (q >> 1) * 64 + ((wave & 1) * 8 + lr) * 4 + (wave >> 1) + 2 * (q & 1);
+        xo[q] = (uint32_t)min(r, a.M - 1 - row0) * (uint32_t)a.ldx + (chunk << 4);
+        if constexpr (SWI) {                                           // (column tiles 0, 1 of a block of 64 gate, 2, 3 up)
+            const int c = min(col0 + (q >> 1) * 32 + ((wave & 1) * 8 + lr) * 2 + (wave >> 1), a.I - 1);
+            wo[q] = (uint32_t)((q & 1) ? a.I + c : c) * (uint32_t)a.ldw + (chunk << 4);
+        } else {
+            wo[q] = (uint32_t)min(r, a.N - 1 - col0) * (uint32_t)a.ldw + (chunk << 4);
+        }
+    }
+    // scales: lane l loads those of x rows l and 64 + l of the wave's 128 and of w rows l and 64 + l of its 128
+    const uint8_t* sxb = (const uint8_t*)a.sx + (int64_t)row0 * a.ldsx;
+    uint32_t so[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        so[h] = (uint32_t)(min(wm * 128 + h * 64 + lane, a.M - 1 - row0) * (int)a.ldsx);
+        const int c = min(col0 + (SWI ? (wn * 2 + h) * 32 + (lane >> 2) * 2 + (lane & 1) : wn * 128 + h * 64 + lane), ncols - 1);
+        so[2 + h] = (uint32_t)(((SWI && (lane & 2) ? a.I + c : c) >> 7) * (int)a.ldsw);
+    }
+    // Position p of the K loop is K tile p; where K ends inside a tile, that tile comes FIRST (position 0) and only the prologue knows about the end of K
+    const int ragged = __builtin_amdgcn_readfirstlane(a.K % FP8_G ? 1 : 0);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + (uint32_t)wave * 1024u);
+    struct From { const uint8_t *x, *w, *sx, *sw; uint32_t d, ds; };
+    auto from = [&](int p, int buf) {                                  // position p to buffer buf (all in scalar registers)
+        const int k = __builtin_amdgcn_readfirstlane(p < ragged ? nk - 1 : p - ragged);
+        auto scalar = [](const uint8_t* p) {
+            const uint64_t u = (uint64_t)p;
+            return (const uint8_t*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)u));
+        };
+        return From{scalar(xbase + (int64_t)k * FP8_G), scalar(wbase + (int64_t)k * FP8_G), scalar(sxb + k), scalar((const uint8_t*)a.sw + k),
+                    (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + (uint32_t)buf * BUF)),
+                    (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 2u * BUF + (uint32_t)buf * 4096u))};
+    };
+    auto dma = [&](auto q, const From& f) {                            // piece q of 16: 8 of x, 8 of w
+        if constexpr (q < 8) dma_to<q * 4096>(xo[q], f.x, f.d);
+        else dma_to<q * 4096>(wo[q - 8], f.w, f.d);
+    };
+    auto dma_scales = [&](auto q, const From& f) { dma_byte_to<q * 256>(so[q], q < 2 ? f.sx : f.sw, f.ds); };      // piece q of 4: 2 of x, 2 of w
+    auto scales4 = [&](int c, int p) { return *reinterpret_cast<const v4i*>(smem + 2 * BUF + (p & 1) * 4096 + wave * 1024 + c * 256 + fi * 16); };      // rows 4 fi .. + 3
+    auto pack = [](const v4i& v) { return (uint32_t)(v[0] | (v[1] << 8) | (v[2] << 16) | (v[3] << 24)); };
+
+    v4f acc[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    v8i af[8], bf[8];
+    uint32_t sx[2], sw[2], nsw[2];
+    auto rd = [&](const uint8_t* t) { return frag(t + fi * FP8_G + ((fg ^ (fi & 7)) << 4), t + fi * FP8_G + (((fg + 4) ^ (fi & 7)) << 4)); };
+    auto xt = [&](int p, int i) { return smem + (p & 1) * BUF + (wm * 128 + i * 16) * FP8_G; };
+    auto wt = [&](int p, int j) { return smem + (p & 1) * BUF + (BM + wn * 128 + j * 16) * FP8_G; };
+    // One K tile: 64 products, two x tiles against the eight w tiles in turn, and behind them the reads whose registers are free.  (The last two tiles load
+    // the last one again, for nobody: one copy of the loop with no branch in it.)
+    constexpr int FREE = 10, LANDED = 34;
+    v4i raw;
+    auto tile = [&](int p) {
+        const From f = from(min(p + 2, nk - 1), p & 1);
+        each<64>([&](auto s_) {
+            constexpr int s = s_, q = s >> 4, j = (s >> 1) & 7, i = q * 2 + (s & 1);
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af[i], acc[i][j], 0, 0, j & 3, (int)sw[j >> 2], i & 3, (int)sx[i >> 2]);
+            if constexpr (s == 0) af[6] = rd(xt(p, 6));
+            if constexpr (s == 2) af[7] = rd(xt(p, 7));
+            if constexpr (s == FREE) {                                           // every wave has read tile p
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+            }
+            if constexpr (s >= FREE && s < FREE + 16) dma(std::integral_constant<int, s - FREE>{}, f);
+            if constexpr (s >= FREE + 16 && s < FREE + 20) dma_scales(std::integral_constant<int, s - FREE - 16>{}, f);
+            if constexpr (s == LANDED) {                                         // tile p + 1 has landed: all but the 20 loads of tile p + 2
+                asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+            }
+            if constexpr (s == 35 || s == 37 || s == 39 || s == 41) af[(s - 35) >> 1] = rd(xt(p + 1, (s - 35) >> 1));                    // (free since 15, 31)
+            if constexpr (s == 43) raw = scales4(2, p + 1);
+            if constexpr (s == 45) nsw[0] = pack(raw), raw = scales4(3, p + 1);
+            if constexpr (s == 47) nsw[1] = pack(raw);
+            if constexpr (q == 3 && (s & 1)) bf[j] = rd(wt(p + 1, j));                                                                    // (free since this product)
+            if constexpr (s == 48 || s == 50) af[s == 48 ? 4 : 5] = rd(xt(p + 1, s == 48 ? 4 : 5));                                      // (since 47)
+            if constexpr (s == 52) raw = scales4(0, p + 1);
+            if constexpr (s == 56) sx[0] = pack(raw), raw = scales4(1, p + 1);                                                            // (since 31)
+            if constexpr (s == 63) sx[1] = pack(raw), sw[0] = nsw[0], sw[1] = nsw[1];
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+
+    // nk >= 2 (the host's choice of this kernel)
+    const From f0 = from(0, 0), f1 = from(1, 1);
+    if (ragged) {                                                      // the chunks behind K read zeros
+        const bool in = (nk - 1) * FP8_G + chunk * 16 < a.K;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            dma_piece_at(in ? xbase + (int64_t)(nk - 1) * FP8_G + xo[q] : (const uint8_t*)&g_zero16, lds0 + (uint32_t)q * 4096u);
+            dma_piece_at(in ? wbase + (int64_t)(nk - 1) * FP8_G + wo[q] : (const uint8_t*)&g_zero16, lds0 + (uint32_t)(BM * FP8_G) + (uint32_t)q * 4096u);
+        }
+    } else {
+        each<16>([&](auto q) { dma(q, f0); });
+    }
+    each<4>([&](auto q) { dma_scales(q, f0); });
+    each<16>([&](auto q) { dma(q, f1); });
+    each<4>([&](auto q) { dma_scales(q, f1); });
+    asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) bf[c] = rd(wt(0, c));
+#pragma unroll
+    for (int c = 0; c < 6; ++c) af[c] = rd(xt(0, c));
+    sx[0] = pack(scales4(0, 0)), sx[1] = pack(scales4(1, 0)), sw[0] = pack(scales4(2, 0)), sw[1] = pack(scales4(3, 0));
+    int p = 0;
+    do tile(p);
+    while (++p < nk);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // (no load into LDS outlives the wave)
+
+    // ---- epilogue.  Lane: row (i >> 2) * 64 + 4 fi + (i & 3) of the wave's 128; of each block h of 64 w rows, columns 16 fg + 4 r + j (SwiGLU: 8 fg + 2 r + j)
+    int elane = lane;
+    asm volatile("" : "+v"(elane));                                   // (what follows from it is not worked out before the K loop and kept: registers)
+    const int ef = elane & 15, eg = elane >> 4, mrow = wm * 128 + ef * 4;
+    constexpr int NC = SWI ? 8 : 16, ND = DT == 3 ? 0 : DT;
+    auto row_of = [&](int i) { return mrow + (i >> 2) * 64 + (i & 3); };
+    auto col_of = [&](int h) { return col0 + (SWI ? (wn * 2 + h) * 32 + eg * 8 : wn * 128 + h * 64 + eg * 16); };
+    auto keep = [&](int i, int h) {                                    // the sums stay where the products left them until here, row by row
+#pragma unroll
+        for (int c = 0; c < 4; ++c) asm volatile("" : "+a"(acc[i][h * 4 + c]));
+    };
+    if constexpr (DT == 3) {                                           // the tile's 128 columns are one group of the result
+        __builtin_amdgcn_s_barrier();                                  // every wave has read its last fragments
+        float* amax = reinterpret_cast<float*>(smem);                  // [2 waves][256 rows]
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float x = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                keep(i, h);
+                float y = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float v = acc[i][h * 4 + 2 + (c & 1)][c >> 1] * silu(acc[i][h * 4 + (c & 1)][c >> 1]);
+                    acc[i][h * 4 + (c & 1)][c >> 1] = v;
+                    y = fmaxf(y, fp8_finite_abs(v));
+                }
+                x = fmaxf(x, col_of(h) < ncols ? y : 0.f);             // (I % 16 == 0: all of the lane's columns or none)
+            }
+            x = fmaxf(x, __shfl_xor(x, 16, 64));
+            x = fmaxf(x, __shfl_xor(x, 32, 64));
+            if (eg == 0) amax[wn * 256 + row_of(i)] = x;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int lrow = row_of(i), m = row0 + lrow;
+            const float x = fmaxf(amax[lrow], amax[256 + lrow]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = acc[i][h * 4 + (c & 1)][c >> 1];
+                uint32_t o[2], code;
+                float s;
+                fp8_quantize_pack<8>(v, x, 0, o, code, s);
+                if (m < a.M) {
+                    if (col_of(h) < ncols) *reinterpret_cast<uint2*>((uint8_t*)a.out + (int64_t)m * a.ldo + col_of(h)) = make_uint2(o[0], o[1]);
+                    if (h == 0 && wn == 0 && eg == 0) ((uint8_t*)a.out_scale)[(int64_t)m * a.ldos + col0 / FP8_G] = (uint8_t)code;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+        // Bias and residual are added whether they are there or not (zeros): only their loads are conditional -- branches around the sums would cost
+        // copies of all 256.  Offsets from the tile's origin in 32 bits: one register per address.
+        const uint8_t* rbase = (const uint8_t*)a.res + ((int64_t)row0 * a.ldr + col0) * 2;
+        uint8_t* obase = (uint8_t*)a.out + ((int64_t)row0 * a.ldo + col0) * 2;
+        auto half = [](const uint4& u, int c) {                        // 16-bit element c of 8
+            const uint32_t w = (c >> 1) == 0 ? u.x : (c >> 1) == 1 ? u.y : (c >> 1) == 2 ? u.z : u.w;
+            return fp_to_f32<ND>((uint16_t)(c & 1 ? w >> 16 : w & 0xffffu));
+        };
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int n = col_of(h);
+            const bool in0 = n < ncols, in1 = NC == 16 && n + 8 < ncols;
+            const uint32_t on = (uint32_t)(n - col0) * 2u;
+            uint4 bias[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+            if (!SWI && a.bias && in0) bias[0] = *reinterpret_cast<const uint4*>((const uint16_t*)a.bias + n);
+            if (!SWI && a.bias && in1) bias[1] = *reinterpret_cast<const uint4*>((const uint16_t*)a.bias + n + 8);
+            uint4 t[8][2];                                             // the residual: 16 loads requested together
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                t[i][0] = t[i][1] = make_uint4(0, 0, 0, 0);
+                if (!SWI && a.res && row0 + row_of(i) < a.M) {
+                    const uint8_t* r = rbase + ((uint32_t)row_of(i) * (uint32_t)a.ldr * 2u + on);
+                    if (in0) t[i][0] = *reinterpret_cast<const uint4*>(r);
+                    if (in1) t[i][1] = *reinterpret_cast<const uint4*>(r + 16);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                keep(i, h);
+                float v[NC];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    if constexpr (SWI) v[c] = acc[i][h * 4 + 2 + (c & 1)][c >> 1] * silu(acc[i][h * 4 + (c & 1)][c >> 1]);
+                    else v[c] = acc[i][h * 4 + (c & 3)][c >> 2] + half(bias[c >> 3], c & 7) + half(t[i][c >> 3], c & 7);
+                }
+                uint8_t* o = obase + ((uint32_t)row_of(i) * (uint32_t)a.ldo * 2u + on);
+                const bool m_in = row0 + row_of(i) < a.M;
+                if (m_in && in0) fp_store8<ND>(o, 0, v);
+                if (m_in && in1) fp_store8<ND>(o, 8, v + NC - 8);
+            }
+        }
+    }
+}
+
+// ================================================================================================================================
 // Few rows (M <= 16 MT): the weights stream once.
 //   * A workgroup owns R neighbouring rows of w (SwiGLU: R gate rows and the R up rows beside them), R chosen so that the grid is one or a few whole
 //     workgroups per CU; its waves take the K blocks in turn (block b to wave b mod waves: side by side they read neighbouring 128 B of the same
@@ -620,12 +888,13 @@ k_fp8_gemm_finish(const GemmArgs a, int swi, int c8 /* threads per row: a multip
 constexpr int CUS = 256;
 
 struct Plan {
-    int rows;                                                          // 16-row tiles of k_fp8_gemm_rows; 0: tile kernel
+    int rows;                                                          // 16-row tiles of k_fp8_gemm_rows; 0: tile kernel, -1: big kernel
     int bm, bn, tiles_m, tiles_n, splits;
     int64_t ldws, ws_bytes;
 };
 
-Plan plan_of(int M, int N, int K, bool swi, int out_type) {
+// wide: rows of out and residual start on 16 bytes
+Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
     Plan p{};
     const int KB = (K + FP8_G - 1) / FP8_G, ncols = swi ? N / 2 : N;
     p.ldws = swi ? 2 * ((ncols + 7) / 8 * 8) : (ncols + 7) / 8 * 8;
@@ -636,6 +905,13 @@ Plan plan_of(int M, int N, int K, bool swi, int out_type) {
         p.rows = M <= 16 ? 1 : M <= 32 ? 2 : 4;
         p.splits = 1;
         p.ws_bytes = out_type == 3 ? (int64_t)M * p.ldws * 4 : 0;
+        return p;
+    }
+    if (kind == 0 && KB >= 2 && out_type != 2 && M > 1024 && wide && ncols % 8 == 0) {
+        p.rows = -1;
+        p.tiles_m = (M + 255) / 256;
+        p.tiles_n = (ncols + (swi ? 127 : 255)) / (swi ? 128 : 256);
+        p.splits = 1;
         return p;
     }
     p.bm = swi ? 64 : 128;
@@ -705,10 +981,29 @@ int32_t launch_rows(const GemmArgs& a, hipStream_t s) {
     }
     return launch_rows_of<KIND, SWI, EXACT, MT, 1>(a, R, s);
 }
+template <bool SWI, int DT>
+int32_t launch_big_of(const GemmArgs& a, hipStream_t s) {
+    const size_t sh = 2 * 512 * FP8_G + 2 * 4 * 1024;
+    static std::atomic<uint64_t> done{0};
+    const int32_t rc = allow_lds(reinterpret_cast<const void*>(&k_fp8_gemm_big<SWI, DT>), sh, done);
+    if (rc != D3D_OK) return rc;
+    hipLaunchKernelGGL((k_fp8_gemm_big<SWI, DT>), dim3((uint32_t)(a.tiles_m * a.tiles_n)), dim3(256), sh, s, a);
+    D3D_LAUNCH_CHECK();
+}
+template <bool SWI>
+int32_t launch_big(const GemmArgs& a, hipStream_t s) {
+    if constexpr (SWI) {
+        if (a.out_type == 3) return launch_big_of<SWI, 3>(a, s);
+    }
+    return a.out_type == 0 ? launch_big_of<SWI, 0>(a, s) : launch_big_of<SWI, 1>(a, s);
+}
 template <int KIND, bool SWI>
 int32_t launch(const GemmArgs& a, int rows, hipStream_t s) {
     // a result that is quantised again is EXACT too while that is free (8 rows of 8192 x 3072: 15.7 us; at 64 rows 32.4 against 25.6)
     const bool exact = a.out_type == 2 || (a.out_type == 3 && rows <= 2);
+    if constexpr (KIND == 0) {
+        if (rows < 0) return launch_big<SWI>(a, s);
+    }
     if (rows == 1) return exact ? launch_rows<KIND, SWI, true, 1>(a, s) : launch_rows<KIND, SWI, false, 1>(a, s);
     if (rows == 2) return exact ? launch_rows<KIND, SWI, true, 2>(a, s) : launch_rows<KIND, SWI, false, 2>(a, s);
     if (rows == 4) return exact ? launch_rows<KIND, SWI, true, 4>(a, s) : launch_rows<KIND, SWI, false, 4>(a, s);
@@ -719,9 +1014,10 @@ int32_t launch(const GemmArgs& a, int rows, hipStream_t s) {
 
 extern "C" {
 
-int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type) {
+int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type, int32_t scale_kind) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return plan_of(M, N, K, swiglu != 0, out_type).ws_bytes;
+    // (the big kernel needs none or less: what the other kernels need covers rows that start anywhere)
+    return std::max(plan_of(M, N, K, swiglu != 0, out_type, scale_kind, true).ws_bytes, plan_of(M, N, K, swiglu != 0, out_type, scale_kind, false).ws_bytes);
 }
 
 int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
@@ -740,8 +1036,9 @@ int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
     if (g->ldx >= (int64_t)1 << 24 || g->ldw >= (int64_t)1 << 24) return bad("d3d_fp8_gemm: rows further than 16 MiB apart");
     if (g->ldsx < 0 || g->ldsw < 0 || g->ldsx >= 1 << 20 || (int64_t)(g->N / FP8_G + 1) * g->ldsw >= 1 << 29) return bad("d3d_fp8_gemm: scale rows too far apart");
     if (swi && (int64_t)g->N * g->ldw >= (int64_t)1 << 32) return bad("d3d_fp8_gemm: SwiGLU weights of 4 GiB and more");
-    const Plan p = plan_of(g->M, g->N, g->K, swi, g->out_type);
-    if (!p.rows && (int64_t)p.tiles_m * p.tiles_n * p.splits >= (int64_t)1 << 31) return bad("d3d_fp8_gemm: too many tiles for one launch");
+    const bool wide = ((uintptr_t)g->out & 15) == 0 && g->ldo % 8 == 0 && g->ldo < 1 << 22 && g->ldr < 1 << 22 && (!g->residual || (((uintptr_t)g->residual & 15) == 0 && g->ldr % 8 == 0)) && ((uintptr_t)g->bias & 15) == 0;
+    const Plan p = plan_of(g->M, g->N, g->K, swi, g->out_type, g->scale_kind, wide);
+    if (p.rows <= 0 && (int64_t)p.tiles_m * p.tiles_n * p.splits >= (int64_t)1 << 31) return bad("d3d_fp8_gemm: too many tiles for one launch");
     if (p.ws_bytes > g->workspace_bytes || (p.ws_bytes && (!g->workspace || ((uintptr_t)g->workspace & 15))))
         return bad("d3d_fp8_gemm: workspace smaller than d3d_fp8_gemm_workspace() or not on 16 bytes");
     GemmArgs a{};

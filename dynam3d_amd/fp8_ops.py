@@ -231,10 +231,10 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float, residual: Optional[to
 
 # ---- products --------------------------------------------------------------------------------------------------------------------------------
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(m, n, k, swiglu, out_type):
+def _workspace_bytes(m, n, k, swiglu, out_type, kind):
     fn = _lib.load().d3d_fp8_gemm_workspace
     fn.restype = C.c_int64
-    return fn(m, n, k, swiglu, out_type)
+    return fn(m, n, k, swiglu, out_type, kind)
 
 
 def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):
@@ -249,7 +249,7 @@ def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):
         ldos = (cols + GROUP - 1) // GROUP
         out_scale = torch.empty((m, ldos), dtype=sx.dtype, device=dev)
         osp = out_scale.data_ptr()
-    nbytes = _workspace_bytes(m, n, k, swiglu, _DT[out_dtype])
+    nbytes = _workspace_bytes(m, n, k, swiglu, _DT[out_dtype], _KIND[sx.dtype])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None      # (stream-ordered: torch's allocator, or the capturing graph's pool)
     bp, rp, ldr = None, None, 0
     if bias is not None:

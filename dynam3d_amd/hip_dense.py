@@ -45,7 +45,7 @@ _lib.register("d3d_fp8_quantize_weight", [vp, vp, vp, i32, i32, i64, i64, i64, i
 _lib.register("d3d_fp8_dequantize", [vp, vp, vp, i32, i32, i64, i64, i64, i32, i32, i32, vp])
 _lib.register("d3d_fp8_rms_norm", [vp, vp, vp, vp, vp, vp, i32, i32, i64, i64, i64, i64, i64, f32, i32, i32, vp])
 _lib.register("d3d_fp8_gemm", [vp])
-_lib.register("d3d_fp8_gemm_workspace", [i32, i32, i32, i32, i32])
+_lib.register("d3d_fp8_gemm_workspace", [i32, i32, i32, i32, i32, i32])
 
 
 def _p(t: Optional[torch.Tensor]):

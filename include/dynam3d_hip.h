@@ -655,7 +655,7 @@ typedef struct d3d_fp8_gemm_args {
     int32_t M, N, K, scale_kind, out_type, swiglu;
     void* stream;
 } d3d_fp8_gemm_args;
-int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type);
+int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type, int32_t scale_kind);
 int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* a);
 
 #ifdef __cplusplus

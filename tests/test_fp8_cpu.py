@@ -88,7 +88,7 @@ def test_c_entry_points_refuse():
         assert lib.d3d_fp8_gemm(C.byref(a)) == -1, kw
         assert b"d3d_fp8_gemm" in lib.d3d_last_error()
     assert lib.d3d_fp8_gemm(None) == -1
-    need = F8._workspace_bytes(4, 64, 4096, 0, 0)
+    need = F8._workspace_bytes(4, 64, 4096, 0, 0, 0)
     if need:
         a = _args(K=4096, ldx=4096, ldw=4096, ldsx=32, ldsw=32, workspace_bytes=need - 1)
         assert lib.d3d_fp8_gemm(C.byref(a)) == -1

@@ -173,7 +173,8 @@ def test_rms_norm_strides():
 
 # ---- products -------------------------------------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 16), (1, 128, 128), (1, 9216, 3072), (2, 3072, 8192), (5, 1003, 1040), (8, 3072, 8192), (16, 32064, 512), (17, 129, 272), (31, 640, 4096),
-          (33, 513, 144), (64, 4096, 1024), (77, 1003, 1040), (127, 255, 384), (128, 256, 128), (129, 257, 2064), (257, 3072, 3072), (577, 4096, 1024), (823, 1024, 4096)]
+          (33, 513, 144), (64, 4096, 1024), (77, 1003, 1040), (127, 255, 384), (128, 256, 128), (129, 257, 2064), (257, 3072, 3072), (577, 4096, 1024), (823, 1024, 4096), (1025, 1, 512), (1100, 2050, 1040),
+          (1281, 511, 528), (2049, 1030, 640), (3000, 3072, 512), (1537, 768, 8192)]
 
 
 @pytest.mark.parametrize("scale", SCALES)
@@ -239,7 +240,7 @@ def swiglu_tol(x, w, k, n, out):
 
 @pytest.mark.parametrize("scale", SCALES)
 @pytest.mark.parametrize("m,i,k", [(1, 16, 16), (1, 8192, 3072), (8, 8192, 3072), (3, 144, 272), (16, 1040, 512), (40, 2064, 400), (64, 128, 128), (65, 272, 1040),
-                                   (129, 4096, 1024), (823, 2048, 640)])
+                                   (129, 4096, 1024), (823, 2048, 640), (1030, 16, 512), (1100, 272, 528), (1281, 1040, 1024), (2500, 2048, 640)])
 def test_linear_swiglu(m, i, k, scale):
     x, w = operands(m, 2 * i, k, scale, m + i)
     out = DTYPES[(m + i // 16) % 3]

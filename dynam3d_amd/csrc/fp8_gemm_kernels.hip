@@ -504,40 +504,47 @@ k_fp8_gemm_big(const GemmArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     v8i af[8], bf[8];
-    uint32_t sx[2], sw[2], nsw[2];
+    uint32_t sx[2], sw[2];
     auto rd = [&](const uint8_t* t) { return frag(t + fi * FP8_G + ((fg ^ (fi & 7)) << 4), t + fi * FP8_G + (((fg + 4) ^ (fi & 7)) << 4)); };
     auto xt = [&](int p, int i) { return smem + (p & 1) * BUF + (wm * 128 + i * 16) * FP8_G; };
     auto wt = [&](int p, int j) { return smem + (p & 1) * BUF + (BM + wn * 128 + j * 16) * FP8_G; };
-    // One K tile: 64 products, two x tiles against the eight w tiles in turn, and behind them the reads whose registers are free.  (The last two tiles load
-    // the last one again, for nobody: one copy of the loop with no branch in it.)
-    constexpr int FREE = 10, LANDED = 34;
+    // One K tile: 64 products, x tiles 0 - 3 and then 4 - 7 against the w tiles in turn: in this order the fragments come free one after the other, and each is
+    // read anew (for the next tile, x tiles 4 - 7 for this one) some 30 products ahead of its use.  Reads and loads are spread evenly: per product (32
+    // cycles) the four waves get one 16-byte read each out of LDS and half a piece out of the caches, so a run of either would stall the products (with
+    // the 20 loads behind one another the kernel took 8 - 10 % longer).  (The last two tiles load the last one again, for nobody: no branch in the loop.)
+    constexpr int FREE = 18, LANDED = 32;
     v4i raw;
     auto tile = [&](int p) {
         const From f = from(min(p + 2, nk - 1), p & 1);
         each<64>([&](auto s_) {
-            constexpr int s = s_, q = s >> 4, j = (s >> 1) & 7, i = q * 2 + (s & 1);
+            constexpr int s = s_, j = (s >> 2) & 7, i = (s >> 5) * 4 + (s & 3);
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af[i], acc[i][j], 0, 0, j & 3, (int)sw[j >> 2], i & 3, (int)sx[i >> 2]);
-            if constexpr (s == 0) af[6] = rd(xt(p, 6));
-            if constexpr (s == 2) af[7] = rd(xt(p, 7));
-            if constexpr (s == FREE) {                                           // every wave has read tile p
+            if constexpr (s == 0) bf[7] = rd(wt(p, 7));
+            if constexpr (s == 2) raw = scales4(1, p);
+            if constexpr (s == 4 || s == 7 || s == 10 || s == 13) af[4 + (s - 4) / 3] = rd(xt(p, 4 + (s - 4) / 3));
+            if constexpr (s == 6) sx[1] = pack(raw);
+            if constexpr (s == FREE) {                                 // every wave has read tile p
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
             }
-            if constexpr (s >= FREE && s < FREE + 16) dma(std::integral_constant<int, s - FREE>{}, f);
-            if constexpr (s >= FREE + 16 && s < FREE + 20) dma_scales(std::integral_constant<int, s - FREE - 16>{}, f);
-            if constexpr (s == LANDED) {                                         // tile p + 1 has landed: all but the 20 loads of tile p + 2
-                asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
+            each<20>([&](auto q) {                                     // piece q behind product FREE + 9 q / 4
+                if constexpr (s == FREE + q * 9 / 4) {
+                    if constexpr (q < 16) dma(q, f);
+                    else dma_scales(std::integral_constant<int, q - 16>{}, f);
+                }
+            });
+            if constexpr (s == LANDED) {                               // tile p + 1 has landed: all but the first loads of tile p + 2
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((LANDED - FREE) * 4 / 9 + 1) : "memory");
                 __builtin_amdgcn_s_barrier();
             }
-            if constexpr (s == 35 || s == 37 || s == 39 || s == 41) af[(s - 35) >> 1] = rd(xt(p + 1, (s - 35) >> 1));                    // (free since 15, 31)
-            if constexpr (s == 43) raw = scales4(2, p + 1);
-            if constexpr (s == 45) nsw[0] = pack(raw), raw = scales4(3, p + 1);
-            if constexpr (s == 47) nsw[1] = pack(raw);
-            if constexpr (q == 3 && (s & 1)) bf[j] = rd(wt(p + 1, j));                                                                    // (free since this product)
-            if constexpr (s == 48 || s == 50) af[s == 48 ? 4 : 5] = rd(xt(p + 1, s == 48 ? 4 : 5));                                      // (since 47)
-            if constexpr (s == 52) raw = scales4(0, p + 1);
-            if constexpr (s == 56) sx[0] = pack(raw), raw = scales4(1, p + 1);                                                            // (since 31)
-            if constexpr (s == 63) sx[1] = pack(raw), sw[0] = nsw[0], sw[1] = nsw[1];
+            if constexpr (s >= 33 && s < 41 && (s - 33) % 2 == 0) af[(s - 33) / 2] = rd(xt(p + 1, (s - 33) / 2));
+            if constexpr (s == 42) raw = scales4(0, p + 1);
+            each<7>([&](auto c) {
+                if constexpr (s == 41 + c * 13 / 4 + (c > 4)) bf[c] = rd(wt(p + 1, c));
+            });
+            if constexpr (s == 46) sx[0] = pack(raw), raw = scales4(2, p + 1);
+            if constexpr (s == 52) sw[0] = pack(raw), raw = scales4(3, p + 1);
+            if constexpr (s == 63) sw[1] = pack(raw);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -560,10 +567,10 @@ k_fp8_gemm_big(const GemmArgs a) {
     asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
     __builtin_amdgcn_s_barrier();
 #pragma unroll
-    for (int c = 0; c < 8; ++c) bf[c] = rd(wt(0, c));
+    for (int c = 0; c < 7; ++c) bf[c] = rd(wt(0, c));
 #pragma unroll
-    for (int c = 0; c < 6; ++c) af[c] = rd(xt(0, c));
-    sx[0] = pack(scales4(0, 0)), sx[1] = pack(scales4(1, 0)), sw[0] = pack(scales4(2, 0)), sw[1] = pack(scales4(3, 0));
+    for (int c = 0; c < 4; ++c) af[c] = rd(xt(0, c));
+    sx[0] = pack(scales4(0, 0)), sw[0] = pack(scales4(2, 0)), sw[1] = pack(scales4(3, 0));
     int p = 0;
     do tile(p);
     while (++p < nk);

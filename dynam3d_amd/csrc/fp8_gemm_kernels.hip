@@ -405,15 +405,16 @@ k_fp8_gemm_tile(const GemmArgs a) {
 
 // ================================================================================================================================
 // Large products, E8M0 scales, results of 8 or 16 bits: 256 x 256 x 128 per workgroup of FOUR waves, 128 x 128 each, one wave per SIMD.
-//   * 64 products of 16x16x128 per wave and K tile on 256 accumulators, out of 16 fragments that stay in registers; a fragment is replaced by the next
-//     K tile's as its last product issues, 12 products (400 cycles) and more ahead of its use.  LDS is read 128 KiB per K tile; with 128 x 64 per
-//     wave (eight waves) it was 192, the two waves of a SIMD met at the barriers, and the matrix pipe was busy 58 % of the time.
+//   * 64 products of 16x16x128 per wave and K tile on 256 accumulators, out of 16 fragments that stay in registers; LDS is read 128 KiB per K tile.  With
+//     128 x 64 per wave (eight waves) it was 192, the two waves of a SIMD met at the barriers, and 8192^3 took 538 us instead of 440.
 //   * Two barriers per K tile: behind the first every wave has read tile p and its buffer takes the DMA of tile p + 2; behind the second tile p + 1
-//     has landed.  A load so has 1.3 tiles (2700 cycles and more) to arrive.
+//     has landed.
 //   * 16x16x128 products: the matrix pipe alone runs 4.3 PFLOP/s on them and 3.6 - 3.9 on 32x32x64 (power), measured on random data.
 //   * Rows are permuted inside blocks of 64: row 4 f + c of a block is row f of tile c, for x and w alike.  A lane then holds 16 NEIGHBOURING columns of a row
 //     (it stores them with no trip through LDS), and the scales of its rows in four tiles are neighbours: they come by DMA too, a dword per row, are
 //     read as one 16-byte piece, and packed into a register of which the instruction picks the byte.
+//   * What bounds it: 8192^3 2.5 PFLOP/s; the matrix pipe is busy 70 % of the cycles, at 1.8 GHz (power); 16 % are waits for loads and at the barriers.  One workgroup
+//     for several output tiles, loading the next one's operands while it stores, gained nothing (172.7 and 171.8 us for 6568 x 9216 x 3072).
 // DT: 0 bf16, 1 fp16, 3 E4M3 + scale (SwiGLU).  Rows of out and residual allow 16-byte accesses, columns come in eights (the host's choice of this kernel).
 // ================================================================================================================================
 // 1 KiB (16 bytes per lane from base + off), or one byte per lane into a dword, to LDS dst + IMM; base and dst in scalar registers.  (m0 is not kept: nothing else
@@ -436,7 +437,7 @@ template <bool SWI, int DT>
 __global__ void __launch_bounds__(256, 1)
 k_fp8_gemm_big(const GemmArgs a) {
     constexpr int BM = 256, BN = 256, BUF = (BM + BN) * FP8_G, OUT_N = SWI ? BN / 2 : BN;
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];     // [2][x 256 x 128 | w 256 x 128], scales [2][4 waves][4][64] dwords
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];     // [2][x 256 x 128 | w 256 x 128], scales [2][x 256 | w 256] dwords
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1, fi = lane & 15, fg = lane >> 4, lr = lane >> 3;
     const int ncols = SWI ? a.I : a.N, nk = a.KB;
@@ -467,15 +468,11 @@ k_fp8_gemm_big(const GemmArgs a) {
             wo[q] = (uint32_t)min(r, a.N - 1 - col0) * (uint32_t)a.ldw + (chunk << 4);
         }
     }
-    // scales: lane l loads those of x rows l and 64 + l of the wave's 128 and of w rows l and 64 + l of its 128
+    // scales: wave v loads those of rows 64 v + lane of x and of w
     const uint8_t* sxb = (const uint8_t*)a.sx + (int64_t)row0 * a.ldsx;
-    uint32_t so[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        so[h] = (uint32_t)(min(wm * 128 + h * 64 + lane, a.M - 1 - row0) * (int)a.ldsx);
-        const int c = min(col0 + (SWI ? (wn * 2 + h) * 32 + (lane >> 2) * 2 + (lane & 1) : wn * 128 + h * 64 + lane), ncols - 1);
-        so[2 + h] = (uint32_t)(((SWI && (lane & 2) ? a.I + c : c) >> 7) * (int)a.ldsw);
-    }
+    const uint32_t sxo = (uint32_t)(min(wave * 64 + lane, a.M - 1 - row0) * (int)a.ldsx);
+    const int sc = min(col0 + (SWI ? wave * 32 + (lane >> 2) * 2 + (lane & 1) : wave * 64 + lane), ncols - 1);
+    const uint32_t swo = (uint32_t)(((SWI && (lane & 2) ? a.I + sc : sc) >> 7) * (int)a.ldsw);
     // Position p of the K loop is K tile p; where K ends inside a tile, that tile comes FIRST (position 0) and only the prologue knows about the end of K
     const int ragged = __builtin_amdgcn_readfirstlane(a.K % FP8_G ? 1 : 0);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + (uint32_t)wave * 1024u);
@@ -488,14 +485,16 @@ k_fp8_gemm_big(const GemmArgs a) {
         };
         return From{scalar(xbase + (int64_t)k * FP8_G), scalar(wbase + (int64_t)k * FP8_G), scalar(sxb + k), scalar((const uint8_t*)a.sw + k),
                     (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + (uint32_t)buf * BUF)),
-                    (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 2u * BUF + (uint32_t)buf * 4096u))};
+                    (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds_addr(smem) + (uint32_t)wave * 256u + 2u * BUF + (uint32_t)buf * 2048u))};
     };
-    auto dma = [&](auto q, const From& f) {                            // piece q of 16: 8 of x, 8 of w
+    auto dma = [&](auto q, const From& f) {                            // piece q of 18: 8 of x, 8 of w, the scales of x and of w
         if constexpr (q < 8) dma_to<q * 4096>(xo[q], f.x, f.d);
-        else dma_to<q * 4096>(wo[q - 8], f.w, f.d);
+        else if constexpr (q < 16) dma_to<q * 4096>(wo[q - 8], f.w, f.d);
+        else if constexpr (q == 16) dma_byte_to<0>(sxo, f.sx, f.ds);
+        else dma_byte_to<1024>(swo, f.sw, f.ds);
     };
-    auto dma_scales = [&](auto q, const From& f) { dma_byte_to<q * 256>(so[q], q < 2 ? f.sx : f.sw, f.ds); };      // piece q of 4: 2 of x, 2 of w
-    auto scales4 = [&](int c, int p) { return *reinterpret_cast<const v4i*>(smem + 2 * BUF + (p & 1) * 4096 + wave * 1024 + c * 256 + fi * 16); };      // rows 4 fi .. + 3
+    // the scales of the lane's four rows in block c of the wave's x (c = 0, 1) or w (2, 3)
+    auto scales4 = [&](int c, int p) { return *reinterpret_cast<const v4i*>(smem + 2 * BUF + (p & 1) * 2048 + (c < 2 ? wm * 2 + c : 4 + wn * 2 + c - 2) * 256 + fi * 16); };
     auto pack = [](const v4i& v) { return (uint32_t)(v[0] | (v[1] << 8) | (v[2] << 16) | (v[3] << 24)); };
 
     v4f acc[8][8];
@@ -511,8 +510,8 @@ k_fp8_gemm_big(const GemmArgs a) {
     // One K tile: 64 products, x tiles 0 - 3 and then 4 - 7 against the w tiles in turn: in this order the fragments come free one after the other, and each is
     // read anew (for the next tile, x tiles 4 - 7 for this one) some 30 products ahead of its use.  Reads and loads are spread evenly: per product (32
     // cycles) the four waves get one 16-byte read each out of LDS and half a piece out of the caches, so a run of either would stall the products (with
-    // the 20 loads behind one another the kernel took 8 - 10 % longer).  (The last two tiles load the last one again, for nobody: no branch in the loop.)
-    constexpr int FREE = 18, LANDED = 32;
+    // the loads behind one another the kernel took 8 - 10 % longer).  (The last two tiles load the last one again, for nobody: no branch in the loop.)
+    constexpr int FREE = 13, LANDED = 32;
     v4i raw;
     auto tile = [&](int p) {
         const From f = from(min(p + 2, nk - 1), p & 1);
@@ -521,20 +520,17 @@ k_fp8_gemm_big(const GemmArgs a) {
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af[i], acc[i][j], 0, 0, j & 3, (int)sw[j >> 2], i & 3, (int)sx[i >> 2]);
             if constexpr (s == 0) bf[7] = rd(wt(p, 7));
             if constexpr (s == 2) raw = scales4(1, p);
-            if constexpr (s == 4 || s == 7 || s == 10 || s == 13) af[4 + (s - 4) / 3] = rd(xt(p, 4 + (s - 4) / 3));
+            if constexpr (s == 4 || s == 6 || s == 8 || s == 10) af[2 + s / 2] = rd(xt(p, 2 + s / 2));
             if constexpr (s == 6) sx[1] = pack(raw);
             if constexpr (s == FREE) {                                 // every wave has read tile p
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
             }
-            each<20>([&](auto q) {                                     // piece q behind product FREE + 9 q / 4
-                if constexpr (s == FREE + q * 9 / 4) {
-                    if constexpr (q < 16) dma(q, f);
-                    else dma_scales(std::integral_constant<int, q - 16>{}, f);
-                }
+            each<18>([&](auto q) {
+                if constexpr (s == FREE + q * 3 - q / 12) dma(q, f);
             });
             if constexpr (s == LANDED) {                               // tile p + 1 has landed: all but the first loads of tile p + 2
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((LANDED - FREE) * 4 / 9 + 1) : "memory");
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((LANDED - FREE) / 3 + 1) : "memory");
                 __builtin_amdgcn_s_barrier();
             }
             if constexpr (s >= 33 && s < 41 && (s - 33) % 2 == 0) af[(s - 33) / 2] = rd(xt(p + 1, (s - 33) / 2));
@@ -561,10 +557,9 @@ k_fp8_gemm_big(const GemmArgs a) {
     } else {
         each<16>([&](auto q) { dma(q, f0); });
     }
-    each<4>([&](auto q) { dma_scales(q, f0); });
-    each<16>([&](auto q) { dma(q, f1); });
-    each<4>([&](auto q) { dma_scales(q, f1); });
-    asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
+    dma(std::integral_constant<int, 16>{}, f0), dma(std::integral_constant<int, 17>{}, f0);
+    each<18>([&](auto q) { dma(q, f1); });
+    asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
     __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int c = 0; c < 7; ++c) bf[c] = rd(wt(0, c));
@@ -990,7 +985,7 @@ int32_t launch_rows(const GemmArgs& a, hipStream_t s) {
 }
 template <bool SWI, int DT>
 int32_t launch_big_of(const GemmArgs& a, hipStream_t s) {
-    const size_t sh = 2 * 512 * FP8_G + 2 * 4 * 1024;
+    const size_t sh = 2 * 512 * FP8_G + 2 * 2048;
     static std::atomic<uint64_t> done{0};
     const int32_t rc = allow_lds(reinterpret_cast<const void*>(&k_fp8_gemm_big<SWI, DT>), sh, done);
     if (rc != D3D_OK) return rc;

@@ -909,18 +909,21 @@ Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
         p.ws_bytes = out_type == 3 ? (int64_t)M * p.ldws * 4 : 0;
         return p;
     }
-    if (kind == 0 && KB >= 2 && out_type != 2 && M > 1024 && wide && ncols % 8 == 0) {
-        p.rows = -1;
-        p.tiles_m = (M + 255) / 256;
-        p.tiles_n = (ncols + (swi ? 127 : 255)) / (swi ? 128 : 256);
-        p.splits = 1;
-        return p;
-    }
     p.bm = swi ? 64 : 128;
     p.bn = 128;                                                        // columns of the result per tile (SwiGLU: 256 rows of w)
     p.tiles_m = (M + p.bm - 1) / p.bm;
     p.tiles_n = (ncols + p.bn - 1) / p.bn;
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    // A round of small tiles (two workgroups per CU) takes as long as one of big tiles (one workgroup), which does twice as much.  us, small : big:
+    // 9216 x 3072, M = 256 30.5 : 39.8, 823 (504 tiles) 39.8 : 40.3, 1024 (576) 65.0 : 40.5; SwiGLU 2 x 8192 x 3072, M = 256 42.1 : 45.8, 512 (512) 50.5 : 46.6.
+    if (kind == 0 && KB >= 2 && out_type != 2 && tiles >= 2 * CUS && wide && ncols % 8 == 0) {
+        p.rows = -1;
+        p.tiles_m = (M + 255) / 256;
+        p.tiles_n = (ncols + (swi ? 127 : 255)) / (swi ? 128 : 256);
+        p.splits = 1;
+        // (The rows of a sparse last round as a product of small tiles with K cut gained nothing: 6568 x 3072 x 8192, 252 + 60 tiles, 171.8 us against 171.0.)
+        return p;
+    }
     // fewer tiles than one round of two workgroups per CU: cut K so that a round is filled, at least 4 K tiles per slice
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * CUS / tiles, KB / 4));
     p.ws_bytes = p.splits > 1 ? (int64_t)p.splits * M * p.ldws * 4 : 0;
@@ -1018,7 +1021,7 @@ extern "C" {
 
 int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type, int32_t scale_kind) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    // (the big kernel needs none or less: what the other kernels need covers rows that start anywhere)
+    // (which kernel is taken depends on where rows start, too: enough for both)
     return std::max(plan_of(M, N, K, swiglu != 0, out_type, scale_kind, true).ws_bytes, plan_of(M, N, K, swiglu != 0, out_type, scale_kind, false).ws_bytes);
 }
 

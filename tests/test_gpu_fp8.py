@@ -350,3 +350,66 @@ def test_streams_and_graph():
             eager = chain(xs[5 - i], xs[0])
             torch.cuda.synchronize()
             assert torch.equal(out, want[i]) and torch.equal(eager, want[5 - i]) and torch.equal(out2, chain(sr, sx))
+
+
+# ---- products of many tiles (256 x 256 per workgroup) ---------------------------------------------------------------------------------------------------
+LARGE = [(2304, 4104, 272), (8200, 1032, 400), (1281, 7000, 640), (4100, 2048, 256), (2100, 8192, 1024), (4097, 3072, 1152)]
+
+
+@pytest.mark.parametrize("out", DTYPES[:2])
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_linear_of_many_tiles(m, n, k, out):
+    x, w = operands(m, n, k, torch.float8_e8m0fnu, m + n)
+    ref, mag = products64(x, w)
+    y = F8.linear(x, w, out_dtype=out)
+    check(y, ref, sum_tol(mag, k, out) + torch.finfo(out).eps / 2 * ref.abs())
+    assert torch.equal(y, F8.linear(x, w, out_dtype=out))
+    b, r = torch.randn(n, generator=gen(4)).to(out).cuda(), torch.randn(m, n, generator=gen(5)).to(out).cuda()
+    want, size = ref + b.to(D) + r.to(D), ref.abs() + b.to(D).abs() + r.to(D).abs()
+    check(F8.linear(x, w, bias=b, residual=r, out_dtype=out), want, sum_tol(mag, k, out) + 2.0 ** -23 * size + torch.finfo(out).eps / 2 * want.abs())
+    wide = torch.zeros(m, n + 8, dtype=out, device="cuda")
+    wide[:, :n] = r
+    assert torch.equal(F8.linear(x, w, residual=wide[:, :n]) if out == torch.bfloat16 else F8.linear(x, w, residual=wide[:, :n], out_dtype=out),
+                       F8.linear(x, w, residual=r, out_dtype=out))
+
+
+@pytest.mark.parametrize("m,i,k", [(1100, 4112, 528), (2050, 2048, 384), (2100, 4096, 1024), (4500, 1040, 272)])
+def test_linear_swiglu_of_many_tiles(m, i, k):
+    test_linear_swiglu(m, i, k, torch.float8_e8m0fnu)
+
+
+def test_a_bad_row_stays_alone_among_many_tiles():
+    m = 4100
+    xf = acts(m, 400, torch.bfloat16, 1)
+    for bad in (0, 2047, 4099):
+        xb = xf.clone()
+        xb[bad, 390] = float("nan")
+        w = F8.quantize_weight(torch.randn(2 * 1024, 400, generator=gen(2)).cuda())
+        y = F8.linear(F8.quantize(xb.cuda()), w)
+        assert bool(y[bad].isnan().all()) and int(y.isnan().any(1).sum()) == 1
+        v = F8.dequantize(F8.linear_swiglu(F8.quantize(xb.cuda()), w, out_dtype=torch.float8_e4m3fn))
+        assert bool(v[bad].isnan().all()) and int(v.isnan().any(1).sum()) == 1
+
+
+def test_many_tiles_on_two_streams_and_in_a_graph():
+    x, w = operands(2100, 8192, 1024, torch.float8_e8m0fnu, 3)
+    z = F8.quantize(acts(2100, 1024, torch.bfloat16, 8).cuda())
+    want = [F8.linear(x, w), F8.linear(z, w)]
+    torch.cuda.synchronize()
+    got, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for j in range(6):
+        with torch.cuda.stream(streams[j % 2]):
+            got.append(F8.linear((x, z)[j % 2], w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(got[j], want[j % 2]) for j in range(6))
+    sx = F8.Fp8(x.data.clone(), x.scale.clone())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = F8.linear(sx, w)
+    for j in range(4):
+        src = (x, z)[j % 2]
+        sx.data.view(torch.uint8).copy_(src.data.view(torch.uint8)), sx.scale.view(torch.uint8).copy_(src.scale.view(torch.uint8))
+        graph.replay()
+        eager = F8.linear(z, w)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[j % 2]) and torch.equal(eager, want[1])

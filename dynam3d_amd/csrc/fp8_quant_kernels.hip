@@ -39,21 +39,19 @@ k_fp8_quant_rows(const void* __restrict__ x, uint8_t* __restrict__ q, void* __re
 }
 
 // ---- RMSNorm [+ residual] -> E4M3 --------------------------------------------------------------------------------------------------------
-// T threads per row (64: four rows per workgroup; 256: one), NCH chunks of 8 elements per thread held in registers.
-template <int DT, int T, int NCH>
+// A workgroup per row, NCH chunks of 8 elements per thread held in registers: the row is read once.
+template <int DT, int NCH>
 __global__ void __launch_bounds__(256)
 k_fp8_rms_norm(const void* __restrict__ x, const void* __restrict__ residual, const float* __restrict__ w, void* __restrict__ sum,
-               uint8_t* __restrict__ q, void* __restrict__ scale, int rows, int D, int64_t ldx, int64_t ldr, int64_t ldsum, int64_t ldq, int64_t lds,
+               uint8_t* __restrict__ q, void* __restrict__ scale, int D, int64_t ldx, int64_t ldr, int64_t ldsum, int64_t ldq, int64_t lds,
                float eps, int kind) {
     __shared__ float part[4];
-    const int lane = threadIdx.x % T;
-    const int row = blockIdx.x * (256 / T) + threadIdx.x / T;
-    if (T == 64 && row >= rows) return;                          // (no barrier below for T = 64; the grid of T = 256 is exact)
+    const int lane = threadIdx.x, row = blockIdx.x;
     float v[NCH][8];
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int k = (c * T + lane) * 8;
+        const int k = (c * 256 + lane) * 8;
         if (k < D) {
             fp_load8<DT>(x, (int64_t)row * ldx + k, v[c]);
         } else {
@@ -64,7 +62,7 @@ k_fp8_rms_norm(const void* __restrict__ x, const void* __restrict__ residual, co
     if (residual) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const int k = (c * T + lane) * 8;
+            const int k = (c * 256 + lane) * 8;
             if (k < D) {
                 float r[8];
                 fp_load8<DT>(residual, (int64_t)row * ldr + k, r);
@@ -88,15 +86,13 @@ k_fp8_rms_norm(const void* __restrict__ x, const void* __restrict__ residual, co
         for (int i = 0; i < 8; ++i) ss += v[c][i] * v[c][i];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-    if constexpr (T == 256) {
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
-        __syncthreads();
-        ss = (part[0] + part[1]) + (part[2] + part[3]);
-    }
+    if ((lane & 63) == 0) part[lane >> 6] = ss;
+    __syncthreads();
+    ss = (part[0] + part[1]) + (part[2] + part[3]);
     const float r = 1.f / sqrtf(ss / (float)D + eps);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int k = (c * T + lane) * 8;
+        const int k = (c * 256 + lane) * 8;
         float a = 0.f;
         if (k < D) {
             float g[8];
@@ -259,15 +255,15 @@ int32_t d3d_fp8_rms_norm(const void* x, const void* residual, const float* w, vo
     const int32_t eb = elem_bytes(dtype);
     if (!x || !q || !scale || !w || ((uintptr_t)w & 15) || !aligned(x, ldx, eb) || !aligned(q, ldq, 1)) return bad("d3d_fp8_rms_norm: rows must start on 16 bytes");
     if (residual && (!sum || !aligned(residual, ldr, eb) || !aligned(sum, ldsum, eb))) return bad("d3d_fp8_rms_norm: residual and sum rows must start on 16 bytes");
-#define ROWS(DT, T, NCH)                                                                                                                              \
-    hipLaunchKernelGGL((k_fp8_rms_norm<DT, T, NCH>), dim3((uint32_t)((rows + 256 / T - 1) / (256 / T))), dim3(256), 0, (hipStream_t)stream, x, residual, w, sum, \
-                       (uint8_t*)q, scale, rows, D, ldx, ldr, ldsum, ldq, lds, eps, scale_kind)
-#define CALL(DT)                                \
-    do {                                        \
-        if (D <= 2048) ROWS(DT, 256, 1);        \
-        else if (D <= 4096) ROWS(DT, 256, 2);   \
-        else if (D <= 8192) ROWS(DT, 256, 4);   \
-        else ROWS(DT, 256, 8);                  \
+#define ROWS(DT, NCH)                                                                                                                            \
+    hipLaunchKernelGGL((k_fp8_rms_norm<DT, NCH>), dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, x, residual, w, sum, (uint8_t*)q, scale, D, ldx, ldr, \
+                       ldsum, ldq, lds, eps, scale_kind)
+#define CALL(DT)                           \
+    do {                                   \
+        if (D <= 2048) ROWS(DT, 1);        \
+        else if (D <= 4096) ROWS(DT, 2);   \
+        else if (D <= 8192) ROWS(DT, 4);   \
+        else ROWS(DT, 8);                  \
     } while (0)
     D3D_BY_DTYPE(dtype, CALL);
 #undef CALL

@@ -66,3 +66,47 @@ extern "C" int32_t d3d_phi3_decode_token(const d3d_phi3_decode_args* a) {
 #undef D3D_TRY
     return D3D_OK;
 }
+
+// The same token with 8-bit linears: eight launches per layer (RMSNorm -> E4M3, qkv, RoPE + attention, quantise, o_proj + residual, RMSNorm -> E4M3,
+// gate_up + SwiGLU -> E4M3, down_proj + residual), of which the four products stream half the bytes of the 16-bit weights.
+extern "C" int32_t d3d_phi3_decode_token_fp8(const d3d_phi3_decode_args* a, const d3d_phi3_decode_fp8* f) {
+    if (!a || !f || a->n_layers <= 0 || a->rows <= 0) return D3D_OK;
+    const int32_t B = a->rows, Hd = a->hidden, H = a->heads, hd = a->head_dim, I = a->mlp, dt = a->dtype, G = 128;
+    if (H * hd != Hd || B > 16 || Hd % 16 || I % 16 || dt < 0 || dt > 1) {
+        d3d_set_error_("d3d_phi3_decode_token_fp8: needs heads * head_dim == hidden (no grouped-query attention), hidden and mlp in multiples of 16, 16-bit activations and rows <= 16");
+        return D3D_EINVAL;
+    }
+    const int64_t hb = (Hd + G - 1) / G, ib = (I + G - 1) / G;
+    void *s = a->stream, *x = a->x;
+    int32_t rc;
+    auto product = [&](const void* in, const void* in_s, int64_t k, int64_t kb, const void* w, const void* ws, int32_t n, void* out, const void* res, bool swiglu) {
+        d3d_fp8_gemm_args g{};
+        g.x = in, g.sx = in_s, g.w = w, g.sw = ws, g.out = out, g.residual = res;
+        g.workspace = f->workspace, g.workspace_bytes = f->workspace_bytes;
+        g.ldx = k, g.ldsx = kb, g.ldw = k, g.ldsw = kb, g.ldr = n, g.ldo = swiglu ? n / 2 : n, g.ldos = ib;
+        g.out_scale = swiglu ? f->act_scale : nullptr;
+        g.M = B, g.N = n, g.K = (int32_t)k, g.out_type = swiglu ? 3 : dt, g.swiglu = swiglu, g.stream = s;
+        return d3d_fp8_gemm(&g);
+    };
+#define D3D_TRY(call)         \
+    do {                      \
+        rc = (call);          \
+        if (rc != D3D_OK) return rc; \
+    } while (0)
+    for (int32_t l = 0; l < a->n_layers; ++l) {
+        D3D_TRY(d3d_fp8_rms_norm(x, nullptr, a->n1[l], nullptr, f->q, f->q_scale, B, Hd, Hd, 0, 0, Hd, hb, a->rms_eps, dt, 0, s));
+        D3D_TRY(product(f->q, f->q_scale, Hd, hb, a->qkv_w[l], f->qkv_s[l], 3 * Hd, a->qkv, nullptr, false));
+        D3D_TRY(d3d_decode_attention(a->qkv, a->prompt_qkv[l], a->cu_seqlens, (char*)a->knew + (int64_t)l * a->cache_layer_stride_bytes,
+                                     (char*)a->vnew + (int64_t)l * a->cache_layer_stride_bytes, a->attn, B, H, hd, a->t_new, a->t_max,
+                                     a->max_prompt_len, a->cos_t, a->sin_t, a->pos, dt, s));                      // RoPE of q, k inside
+        D3D_TRY(d3d_fp8_quantize(a->attn, f->q, f->q_scale, B, Hd, Hd, Hd, hb, dt, 0, s));
+        D3D_TRY(product(f->q, f->q_scale, Hd, hb, a->o_w[l], f->o_s[l], Hd, x, x, false));                        // + residual, in place
+        D3D_TRY(d3d_fp8_rms_norm(x, nullptr, a->n2[l], nullptr, f->q, f->q_scale, B, Hd, Hd, 0, 0, Hd, hb, a->rms_eps, dt, 0, s));
+        D3D_TRY(product(f->q, f->q_scale, Hd, hb, a->gate_up_w[l], f->gate_up_s[l], 2 * I, a->act, nullptr, true));
+        D3D_TRY(product(a->act, f->act_scale, I, ib, a->down_w[l], f->down_s[l], Hd, x, x, false));
+    }
+    D3D_TRY(d3d_norm(x, a->norm_w, nullptr, a->h, B, Hd, Hd, Hd, a->rms_eps, 1, dt, s));
+    D3D_TRY(d3d_gemm_nt(a->h, a->lm_head_w, a->logits, nullptr, nullptr, B, a->vocab, Hd, Hd, Hd, a->vocab, dt, 0, s));
+#undef D3D_TRY
+    return D3D_OK;
+}

@@ -232,9 +232,15 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float, residual: Optional[to
 # ---- products --------------------------------------------------------------------------------------------------------------------------------
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(m, n, k, swiglu, out_type, kind):
+    """(a function of the sizes and types alone)"""
     fn = _lib.load().d3d_fp8_gemm_workspace
     fn.restype = C.c_int64
     return fn(m, n, k, swiglu, out_type, kind)
+
+
+def workspace_bytes(m: int, n: int, k: int, swiglu: bool = False, out_dtype: torch.dtype = torch.bfloat16, scale_dtype: torch.dtype = E8M0) -> int:
+    """Scratch that a C caller of `d3d_fp8_gemm` has to bring for a product of x (m, k) with w (n, k)."""
+    return _workspace_bytes(m, n, k, int(swiglu), _DT[out_dtype], _KIND[scale_dtype])
 
 
 def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):

@@ -27,6 +27,7 @@ _lib.register("d3d_swiglu", [vp, vp, i64, i32, i32, vp])
 _lib.register("d3d_resize_normalize", [vp, vp, i32, i32, i32, i32, vp, vp, vp])
 _lib.register("d3d_decode_attention", [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp])
 _lib.register("d3d_phi3_decode_token", [vp])
+_lib.register("d3d_phi3_decode_token_fp8", [vp, vp])
 _lib.register("d3d_phi3_decode_status", [vp])
 _lib.register("d3d_patchify", [vp, vp, i32, i32, i32, i32, i32, vp])
 _lib.register("d3d_vit_embed_ln", [vp, vp, vp, vp, vp, vp, i32, i32, i32, f32, i32, vp])
@@ -71,6 +72,12 @@ class Phi3DecodeArgs(C.Structure):
                 ("prompt_qkv", C.POINTER(C.c_void_p)), ("cu_seqlens", C.c_void_p), ("knew", C.c_void_p), ("vnew", C.c_void_p),
                 ("cache_layer_stride_bytes", C.c_int64), ("t_new", C.c_int32), ("t_max", C.c_int32), ("max_prompt_len", C.c_int32),
                 ("stream", C.c_void_p)]
+
+
+class Phi3DecodeFp8(C.Structure):
+    """ctypes mirror of `d3d_phi3_decode_fp8` (include/dynam3d_hip.h)."""
+    _fields_ = ([(n, C.POINTER(C.c_void_p)) for n in ("qkv_s", "o_s", "gate_up_s", "down_s")]
+                + [(n, C.c_void_p) for n in ("q", "q_scale", "act_scale", "workspace")] + [("workspace_bytes", C.c_int64)])
 
 
 def ptr_array(tensors):
@@ -190,6 +197,11 @@ class HipDense:
         """All launches of one KV-cache decode token, issued from C++ (d3d_phi3_decode_token)."""
         args.stream = self._stream()
         _lib.check(self.lib.d3d_phi3_decode_token(C.byref(args)))
+
+    def phi3_decode_token_fp8(self, args: "Phi3DecodeArgs", fp8: "Phi3DecodeFp8"):
+        """The same token with 8-bit linears (d3d_phi3_decode_token_fp8)."""
+        args.stream = self._stream()
+        _lib.check(self.lib.d3d_phi3_decode_token_fp8(C.byref(args), C.byref(fp8)))
 
     def phi3_decode_status(self):
         """Synchronises the stream and raises if a grid barrier of the persistent decode kernel timed out (d3d_phi3_decode_status)."""

@@ -139,6 +139,7 @@ class PolicyConfig:
     llm: Phi3Config = field(default_factory=Phi3Config)
     clip_dtype: torch.dtype = torch.float16      # reference: clip.load(..., device=cuda) -> fp16 (resnet_encoders.py:260)
     llava_dtype: torch.dtype = torch.bfloat16    # reference: torch_dtype=torch.bfloat16 (VLN-POL:125)
+    llm_quant: Optional[str] = None              # "fp8": the language model's linears on 8-bit operands (towers.Phi3Decoder)
     depth_quirk: bool = False                    # True reproduces `observations['depth'][b][i]` row indexing
     compat: str = "reference"
     hip_dense: bool = True                       # on a GPU the towers run on the hand-written HIP kernels (dense_ops.enable_hip_kernels);
@@ -186,7 +187,7 @@ class Dynam3D_VLN(RefreshOnChange):
         for name, (din, dh, dout) in zip(PREFIX_MLPS, ((6, hidden, hidden), (3, width, width), (3, width, width),
                                                        (2 * width, hidden, hidden), (2 * width, hidden, hidden))):        # VLN-POL:83-111
             setattr(self, name, make_prefix_mlp(din, dh, dout, self.device, sd, name + "."))
-        self.llava = LlavaModel(sd, cfg.vit, cfg.llm, cfg.llava_dtype, device)
+        self.llava = LlavaModel(sd, cfg.vit, cfg.llm, cfg.llava_dtype, device, cfg.llm_quant)
         self.depth_encoder = depth_encoder if depth_encoder is not None else DepthEncoderSlot()
         self.space_pool_depth = torch.nn.Sequential(torch.nn.AdaptiveAvgPool2d((1, 1)), torch.nn.Flatten(start_dim=2))   # VLN-POL:144
         self.rgb_encoder = ClipEncoder(sd, cfg.vit, cfg.clip_dtype, device)

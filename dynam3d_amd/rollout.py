@@ -124,6 +124,7 @@ def main():
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--stop-mod", type=int, default=7, help="an episode stops when its argmax token is divisible by this (huge = never: full-length episodes)")
     ap.add_argument("--per-rank", action="store_true", help="every rank prints its own wall / CPU seconds (host-side load when ranks share a host)")
+    ap.add_argument("--llm-quant", choices=["fp8"], default=None, help="run the language model's linears on 8-bit operands (default: its 16-bit type)")
     ap.add_argument("--logits-only", action="store_true", help="open-loop episodes, forward_logits only (the headline metric's step); default: the closed loop with generation")
     ap.add_argument("--new-tokens", type=int, default=20, help="max_new_tokens of the generation (VLN-POL:463: 20)")
     ap.add_argument("--grammar-stop-mod", type=int, default=24, help="ActionGrammarTokenizer: ~2 of this many sentences end an episode")
@@ -134,7 +135,7 @@ def main():
     torch.cuda.set_device(local)
     dev = f"cuda:{local}"
     D.enable_hip_kernels(["all"])
-    cfg = PolicyConfig()
+    cfg = PolicyConfig(llm_quant=a.llm_quant)
     from .policy import ActionGrammarTokenizer
     net = Dynam3D_VLN(cfg, synth_policy_weights(cfg, a.seed, device=dev), device=dev, batch_size=a.episodes_per_rank, max_steps=a.max_steps + 1,
                       tokenizer=None if a.logits_only else ActionGrammarTokenizer(cfg.llm.vocab, stop_mod=a.grammar_stop_mod))

@@ -23,6 +23,7 @@ import torch
 from torch import nn
 
 from . import dense_ops as D
+from . import fp8_ops as F8
 from .modules import ParamTree, install_param, own_copy
 from .profiling import TIMER
 
@@ -253,8 +254,16 @@ class LlavaVisionTower(_VitTrunk):
 # Phi-3-mini decoder prefill
 # ---------------------------------------------------------------------------------------------------
 class Phi3Decoder:
-    def __init__(self, sd: Dict[str, torch.Tensor], cfg: Phi3Config = Phi3Config(), dtype=torch.bfloat16, device="cuda"):
-        self.cfg, self.dtype, self.device = cfg, dtype, torch.device(device)
+    """`quant`: None -- weights and activations in `dtype` -- or "fp8": the four linears of every layer on E4M3 operands (`fp8_ops`: weights with one
+    power-of-two scale per 128 x 128 block, quantised once at load; activations with one per row and 128 columns, quantised where they are made: by the
+    RMSNorm, behind the attention, by the SwiGLU product).  The residual stream, the attention with its KV cache, the embedding and lm_head stay in `dtype`."""
+
+    def __init__(self, sd: Dict[str, torch.Tensor], cfg: Phi3Config = Phi3Config(), dtype=torch.bfloat16, device="cuda", quant: Optional[str] = None):
+        if quant not in (None, "fp8"):
+            raise ValueError(f"Phi3Decoder: quant is None or 'fp8', not {quant!r}")
+        if quant and (cfg.hidden % 16 or cfg.mlp % 16 or (cfg.heads * cfg.head_dim) % 16):
+            raise ValueError("Phi3Decoder: 8-bit linears need hidden, mlp and heads * head_dim in multiples of 16")
+        self.cfg, self.dtype, self.device, self.quant = cfg, dtype, torch.device(device), quant
         self._rope_cache = {}
         self.load(sd)
 
@@ -267,7 +276,8 @@ class Phi3Decoder:
         m = "language_model.model"
         self.embed_w = t(sd[m + ".embed_tokens.weight"])
         # gate/up rows interleaved per 16 for the fused SwiGLU GEMM epilogue (only when the HIP GEMM is active)
-        self.interleave_gu = D.BACKEND["linear"] == "hip" and cfg.mlp % 16 == 0 and dtype != torch.float32     # (float32 verification mode: plain rows)
+        # (float32 verification mode and 8-bit linears: plain rows)
+        self.interleave_gu = D.BACKEND["linear"] == "hip" and cfg.mlp % 16 == 0 and dtype != torch.float32 and not self.quant
         self.layers = []
         for i in range(cfg.layers):
             p = f"{m}.layers.{i}"
@@ -275,11 +285,24 @@ class Phi3Decoder:
             if self.interleave_gu:
                 from .hip_dense import interleave_gate_up
                 gu = interleave_gate_up(gu)
-            self.layers.append(dict(qkv_w=t(sd[p + ".self_attn.qkv_proj.weight"]), o_w=t(sd[p + ".self_attn.o_proj.weight"]),
-                                    gu_w=gu, down_w=t(sd[p + ".mlp.down_proj.weight"]),
+            q = (lambda w: F8.quantize_weight(w)) if self.quant else (lambda w: w)
+            self.layers.append(dict(qkv_w=q(t(sd[p + ".self_attn.qkv_proj.weight"])), o_w=q(t(sd[p + ".self_attn.o_proj.weight"])),
+                                    gu_w=q(gu), down_w=q(t(sd[p + ".mlp.down_proj.weight"])),
                                     n1=f(sd[p + ".input_layernorm.weight"]), n2=f(sd[p + ".post_attention_layernorm.weight"])))
         self.norm_w = f(sd[m + ".norm.weight"])
         self.lm_head_w = t(sd["language_model.lm_head.weight"])
+
+    def _norm(self, x, w):
+        """RMSNorm of rows x (T, hidden): what `_proj` and `_gate_up` take."""
+        return F8.rms_norm(x, w, self.cfg.rms_eps) if self.quant else D.rms_norm(x, w, self.cfg.rms_eps)
+
+    def _proj(self, h, w, residual=None):
+        if not self.quant:
+            return D.linear(h, w, None, residual=residual)
+        return F8.linear(h if isinstance(h, F8.Fp8) else F8.quantize(h), w, residual=residual, out_dtype=self.dtype)
+
+    def _gate_up(self, h, w):
+        return F8.linear_swiglu(h, w, out_dtype=F8.E4M3) if self.quant else D.linear_swiglu(h, w, self.interleave_gu)
 
     PRUNE_LAST_LAYER = True            # prefill_logits_packed: the last layer's o_proj / MLP on the B last rows only
     MAX_DECODE_ROWS = 16          # k_gemm_skinny: M <= 16
@@ -374,8 +397,7 @@ class Phi3Decoder:
         the per-layer teacher-forced parity tests (tests/test_gpu_depth_parity.py)."""
         c, L = self.cfg, self.layers[li]
         Tp, Ht = x.shape[0], c.heads + 2 * c.kv_heads
-        h = D.rms_norm(x, L["n1"], c.rms_eps)
-        qkv = D.linear(h, L["qkv_w"], None)
+        qkv = self._proj(self._norm(x, L["n1"]), L["qkv_w"])
         fuse_q = self.FUSE_ROPE_Q and D.can_fuse_rope_q(self.dtype)
         if fuse_q:
             # keys rotated in place (the KV cache keeps rotated keys), queries rotated inside the attention kernel: half of k_rope's traffic
@@ -390,19 +412,19 @@ class Phi3Decoder:
         a = a.view(Tp, c.heads * c.head_dim)
         if prune:
             a, x = a[ctx["last_rows"]].contiguous(), x[ctx["last_rows"]].contiguous()
-        x = D.linear(a, L["o_w"], None, residual=x)
-        h = D.rms_norm(x, L["n2"], c.rms_eps)
+        x = self._proj(a, L["o_w"], residual=x)
+        h = self._norm(x, L["n2"])
         if h.shape[0] == Tp and li % self.TIME_EVERY == 0:
             # bench.py's roofline launch (full-row GEMMs only), HIP-event timed in every TIME_EVERY-th layer: an event pair costs ~6 us on
             # the stream and the bracket below as much again -- timing all 31 full-row launches of a step put 0.4 ms of instrumentation
             # into the step it measures (D3D_BENCH_TIME_EVERY=1: every layer, as rounds 1-4 did)
             with TIMER.range("phi3.gate_up_proj", rows=ctx["cu_h"][-1], rows_launched=Tp):
-                act = D.linear_swiglu(h, L["gu_w"], self.interleave_gu)
+                act = self._gate_up(h, L["gu_w"])
             with TIMER.range("phi3.event_pair_overhead"):                   # an EMPTY bracket right behind it: what two event records
                 pass                                                        # cost on this stream at this point (bench.py subtracts it)
         else:
-            act = D.linear_swiglu(h, L["gu_w"], self.interleave_gu)
-        return D.linear(act, L["down_w"], None, residual=x)
+            act = self._gate_up(h, L["gu_w"])
+        return self._proj(act, L["down_w"], residual=x)
 
     @torch.no_grad()
     def final_logits(self, last: torch.Tensor) -> torch.Tensor:
@@ -501,17 +523,20 @@ class Phi3Decoder:
     def _decode_runner(self, B, kv, cu, side, cos, sin, max_prompt_len):
         """One decode token = one C call (d3d_phi3_decode_token issues the ~260 launches from C++; from Python they cost more
         host time than the 8-row kernels run).  Returns run(x, pos, t_new) -> logits (B, vocab) float32."""
-        from .hip_dense import HipDense, Phi3DecodeArgs, ptr_array
+        from .hip_dense import HipDense, Phi3DecodeArgs, Phi3DecodeFp8, ptr_array
         c = self.cfg
-        if not (self.interleave_gu and B <= 16):
-            raise RuntimeError("KV-cache decode needs the HIP GEMM backend (interleaved gate/up weights) and <= 16 sequences")
+        if not ((self.interleave_gu or self.quant and D.BACKEND["linear"] == "hip" and self.dtype != torch.float32) and B <= 16):
+            raise RuntimeError("KV-cache decode needs the HIP GEMM backend (interleaved gate/up weights), 16-bit activations and <= 16 sequences")
         hdn = HipDense()
         dev, dt = self.device, self.dtype
         buf = dict(h=torch.empty((B, c.hidden), dtype=dt, device=dev), qkv=torch.empty((B, 3 * c.hidden), dtype=dt, device=dev),
-                   attn=torch.empty((B, c.hidden), dtype=dt, device=dev), act=torch.empty((B, c.mlp), dtype=dt, device=dev),
+                   attn=torch.empty((B, c.hidden), dtype=dt, device=dev), act=torch.empty((B, c.mlp), dtype=F8.E4M3 if self.quant else dt, device=dev),
                    logits=torch.empty((B, c.vocab), dtype=dt, device=dev))
         if getattr(self, "_w_arrays", None) is None:                            # weight pointer tables: built once per decoder
-            self._w_arrays = {k: ptr_array([L[k] for L in self.layers]) for k in ("qkv_w", "o_w", "gu_w", "down_w", "n1", "n2")}
+            data = lambda w: w.data if isinstance(w, F8.Fp8) else w
+            self._w_arrays = {k: ptr_array([data(L[k]) for L in self.layers]) for k in ("qkv_w", "o_w", "gu_w", "down_w", "n1", "n2")}
+            if self.quant:
+                self._w_arrays.update({k[:-1] + "s": ptr_array([L[k].scale for L in self.layers]) for k in ("qkv_w", "o_w", "gu_w", "down_w")})
         wa = self._w_arrays
         kv_arr = ptr_array(kv)
         a = Phi3DecodeArgs()
@@ -527,9 +552,21 @@ class Phi3Decoder:
         a.t_max, a.max_prompt_len = side.shape[3], max_prompt_len
         keep = (buf, kv_arr, kv, side, cos, sin, cu)                           # referenced by raw pointers above
 
+        f = None
+        if self.quant:
+            groups = lambda k: (k + F8.GROUP - 1) // F8.GROUP
+            buf.update(q=torch.empty((B, c.hidden), dtype=F8.E4M3, device=dev), q_scale=torch.empty((B, groups(c.hidden)), dtype=F8.E8M0, device=dev),
+                       act_scale=torch.empty((B, groups(c.mlp)), dtype=F8.E8M0, device=dev),
+                       workspace=torch.empty(F8.workspace_bytes(B, 2 * c.mlp, c.hidden, swiglu=True, out_dtype=F8.E4M3), dtype=torch.uint8, device=dev))
+            f = Phi3DecodeFp8(wa["qkv_s"], wa["o_s"], wa["gu_s"], wa["down_s"], *(buf[k].data_ptr() for k in ("q", "q_scale", "act_scale", "workspace")),
+                              buf["workspace"].numel())
+
         def run(x, pos, t_new):
             a.x, a.pos, a.t_new = x.data_ptr(), pos.data_ptr(), t_new
-            hdn.phi3_decode_token(a)
+            if f is None:
+                hdn.phi3_decode_token(a)
+            else:
+                hdn.phi3_decode_token_fp8(a, f)
             return buf["logits"].float() if keep else None
         run.status = hdn.phi3_decode_status
         return run
@@ -543,20 +580,20 @@ class Phi3Decoder:
         x = inputs_embeds.to(self.dtype).contiguous()
         cos, sin = self._rope(S)
         for L in self.layers:
-            h = D.rms_norm(x, L["n1"], c.rms_eps)
-            qkv = D.linear(h.view(B * S, Hd), L["qkv_w"], None).view(B, S, c.heads + 2 * c.kv_heads, c.head_dim)
+            x = x.view(B * S, Hd)
+            qkv = self._proj(self._norm(x, L["n1"]), L["qkv_w"]).view(B, S, c.heads + 2 * c.kv_heads, c.head_dim)
             qkv = D.rope_qk_(qkv, c.heads + c.kv_heads, cos, sin)
             if c.kv_heads == c.heads:
                 a = D.attention_qkv(qkv, c.heads, causal=True)
             else:
                 q, k, v = qkv[:, :, :c.heads], qkv[:, :, c.heads:c.heads + c.kv_heads], qkv[:, :, c.heads + c.kv_heads:]
                 a = D.attention(q, k, v, causal=True)
-            x = D.linear(a.reshape(B * S, c.heads * c.head_dim), L["o_w"], None, residual=x.view(B * S, Hd)).view(B, S, Hd)
-            h = D.rms_norm(x, L["n2"], c.rms_eps)
+            x = self._proj(a.reshape(B * S, c.heads * c.head_dim), L["o_w"], residual=x)
+            h = self._norm(x, L["n2"])
             with TIMER.range("phi3.gate_up_proj"):
-                act = D.linear_swiglu(h.view(B * S, Hd), L["gu_w"], self.interleave_gu)
-            x = D.linear(act, L["down_w"], None, residual=x.view(B * S, Hd)).view(B, S, Hd)
-        last = x[torch.arange(B, device=x.device), (lengths.to(x.device).long() - 1)]
+                act = self._gate_up(h, L["gu_w"])
+            x = self._proj(act, L["down_w"], residual=x).view(B, S, Hd)
+        last = x.view(B, S, Hd)[torch.arange(B, device=x.device), (lengths.to(x.device).long() - 1)]
         last = D.rms_norm(last, self.norm_w, c.rms_eps)
         return D.linear(last, self.lm_head_w, None).float()
 
@@ -635,7 +672,7 @@ class LlavaModel(nn.Module):
     `vision` (`LlavaVisionTower`) and `lm` (`Phi3Decoder`) are the compute objects over them.  Trainable flags as the reference sets
     them: vision tower and projector frozen (VLN-POL:152-155), the language model trainable."""
 
-    def __init__(self, sd: Dict[str, torch.Tensor], vit: VitConfig, llm: Phi3Config, dtype=torch.bfloat16, device="cuda"):
+    def __init__(self, sd: Dict[str, torch.Tensor], vit: VitConfig, llm: Phi3Config, dtype=torch.bfloat16, device="cuda", llm_quant: Optional[str] = None):
         super().__init__()
         dev = torch.device(device)
         st = lambda n: own_copy(sd[n], dev, dtype)
@@ -645,7 +682,7 @@ class LlavaModel(nn.Module):
             self._add(n, st(n), False)
         flat = self.flat()
         self.vision = LlavaVisionTower(flat, vit, dtype, dev)
-        self.lm = Phi3Decoder(flat, llm, dtype, dev)
+        self.lm = Phi3Decoder(flat, llm, dtype, dev, quant=llm_quant)
         self._sig = self._signature()
 
     def _add(self, dotted, tensor, requires_grad):

@@ -658,6 +658,21 @@ typedef struct d3d_fp8_gemm_args {
 int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type, int32_t scale_kind);
 int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* a);
 
+/* The decode token of d3d_phi3_decode_token with 8-bit linears: `args` as there, but qkv_w / o_w / gate_up_w / down_w are E4M3 (gate_up_w PLAIN: gate rows, then up
+ * rows), act is (rows, mlp) E4M3 and h is used for the final norm only (lm_head stays in the activations' dtype); `f`: the E8M0 scales per 128 x 128 block
+ * (ceil(N / 128), ceil(K / 128)), and scratch.  hidden and mlp are multiples of 16, rows <= 16. */
+typedef struct d3d_phi3_decode_fp8 {
+    const void* const* qkv_s;         /* [n_layers] host arrays of device pointers */
+    const void* const* o_s;
+    const void* const* gate_up_s;
+    const void* const* down_s;
+    void *q, *q_scale;                /* (rows, hidden) E4M3, (rows, ceil(hidden / 128)) E8M0 */
+    void* act_scale;                  /* (rows, ceil(mlp / 128)) */
+    void* workspace;                  /* d3d_fp8_gemm_workspace(rows, 2 * mlp, hidden, 1, 3, 0) bytes */
+    int64_t workspace_bytes;
+} d3d_phi3_decode_fp8;
+int32_t d3d_phi3_decode_token_fp8(const d3d_phi3_decode_args* args, const d3d_phi3_decode_fp8* f);
+
 #ifdef __cplusplus
 }
 #endif

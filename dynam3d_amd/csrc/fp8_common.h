@@ -51,8 +51,22 @@ __device__ __forceinline__ void fp8_quantize_pack(const float* v, float amax, in
     } else {
         code = 0;
         s = fmaxf(amax / 448.f, 0x1p-126f);
+        if (s >= 0x1p-80f) {
+            // v / s correctly rounded, without a division per value: r = 1 / s rounded, t = v r is off by two steps at most, and each
+            // t += r (v - t s), the remainder exact, makes it the neighbour and then the nearest (Markstein).  (The remainder of a v that does not round
+            // to 0 in E4M3, |v| >= 2^-10 s, is far from the denormals here.)  fp16 4617 x 4112 with float32 scales: 30.2 us with divisions and the threads of
+            // the time, 22.4; quantising 6568 x 3072 18.5 -> 15.9.
+            const float r = 1.f / s;
 #pragma unroll
-        for (int i = 0; i < N; ++i) t[i] = v[i] / s;
+            for (int i = 0; i < N; ++i) {
+                t[i] = v[i] * r;
+                t[i] = __builtin_fmaf(__builtin_fmaf(-t[i], s, v[i]), r, t[i]);
+                t[i] = __builtin_fmaf(__builtin_fmaf(-t[i], s, v[i]), r, t[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) t[i] = v[i] / s;
+        }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)

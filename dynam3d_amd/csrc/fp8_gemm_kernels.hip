@@ -1043,7 +1043,7 @@ int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
     if (swi && (int64_t)g->N * g->ldw >= (int64_t)1 << 32) return bad("d3d_fp8_gemm: SwiGLU weights of 4 GiB and more");
     const bool wide = ((uintptr_t)g->out & 15) == 0 && g->ldo % 8 == 0 && g->ldo < 1 << 22 && g->ldr < 1 << 22 && (!g->residual || (((uintptr_t)g->residual & 15) == 0 && g->ldr % 8 == 0)) && ((uintptr_t)g->bias & 15) == 0;
     const Plan p = plan_of(g->M, g->N, g->K, swi, g->out_type, g->scale_kind, wide);
-    if (p.rows <= 0 && (int64_t)p.tiles_m * p.tiles_n * p.splits >= (int64_t)1 << 31) return bad("d3d_fp8_gemm: too many tiles for one launch");
+    if (p.rows <= 0 && (int64_t)p.tiles_m * p.tiles_n * p.splits >= (int64_t)1 << 24) return bad("d3d_fp8_gemm: too many tiles for one launch");
     if (p.ws_bytes > g->workspace_bytes || (p.ws_bytes && (!g->workspace || ((uintptr_t)g->workspace & 15))))
         return bad("d3d_fp8_gemm: workspace smaller than d3d_fp8_gemm_workspace() or not on 16 bytes");
     GemmArgs a{};

@@ -188,7 +188,7 @@ int32_t bad(const char* msg) {
 
 bool aligned(const void* p, int64_t ld, int32_t elem_bytes) { return ((uintptr_t)p & 15) == 0 && (ld * elem_bytes) % 16 == 0; }
 int32_t elem_bytes(int32_t dtype) { return dtype == 2 ? 4 : 2; }
-bool blocks_ok(int64_t n) { return n > 0 && n < (int64_t)1 << 31; }
+bool blocks_ok(int64_t n, int64_t threads = 256) { return n * threads < (int64_t)1 << 32; }        // (a launch has less than 2^32 threads)
 
 #define D3D_BY_DTYPE(dtype, CALL) \
     do {                          \
@@ -259,6 +259,7 @@ int32_t d3d_fp8_rms_norm(const void* x, const void* residual, const float* w, vo
     if (!x || !q || !scale || !w || ((uintptr_t)w & 15) || !aligned(x, ldx, eb) || !aligned(q, ldq, 1)) return bad("d3d_fp8_rms_norm: rows must start on 16 bytes");
     if (residual && (!sum || !aligned(residual, ldr, eb) || !aligned(sum, ldsum, eb))) return bad("d3d_fp8_rms_norm: residual and sum rows must start on 16 bytes");
     const int32_t nch = D <= 4096 ? 2 : D <= 6144 ? 3 : 4, threads = (D + nch * 512 - 1) / (nch * 512) * 64;
+    if (!blocks_ok(rows, threads)) return bad("d3d_fp8_rms_norm: too many rows for one launch");
 #define ROWS(DT, NCH)                                                                                                                            \
     hipLaunchKernelGGL((k_fp8_rms_norm<DT, NCH>), dim3((uint32_t)rows), dim3(threads), 0, (hipStream_t)stream, x, residual, w, sum, (uint8_t*)q, scale, D, ldx, \
                        ldr, ldsum, ldq, lds, eps, scale_kind)

@@ -102,3 +102,23 @@ def test_c_entry_points_refuse():
     assert lib.d3d_fp8_dequantize(p, p, p, 4, 32, 32, 1, 32, 64, 0, 0, None) == -1
     assert lib.d3d_fp8_rms_norm(p, None, p, None, p, p, 4, 16400, 16400, 0, 0, 16400, 1, 1e-5, 0, 0, None) == -1
     assert lib.d3d_fp8_rms_norm(p, p, p, None, p, p, 4, 32, 32, 32, 32, 32, 1, 1e-5, 0, 0, None) == -1
+
+
+def test_c_entry_points_refuse_more_than_a_launch_holds():
+    lib, p, many = _lib.load(), 1 << 20, (1 << 31) - 1
+    assert lib.d3d_fp8_quantize(p, p, p, many, 4096, 4096, 4096, 32, 0, 0, None) == -1
+    assert lib.d3d_fp8_dequantize(p, p, p, many, 4096, 4096, 32, 4096, 1, 0, 0, None) == -1
+    assert lib.d3d_fp8_rms_norm(p, None, p, None, p, p, many, 4096, 4096, 0, 0, 4096, 32, 1e-5, 0, 0, None) == -1
+    a = _args(M=many, N=1 << 20, ldo=1 << 20, ldr=0)
+    assert lib.d3d_fp8_gemm(C.byref(a)) == -1
+
+
+def test_decode_token_refusals():
+    from dynam3d_amd.hip_dense import Phi3DecodeArgs, Phi3DecodeFp8
+    lib = _lib.load()
+    good = dict(n_layers=1, rows=2, hidden=192, heads=2, head_dim=96, mlp=256, vocab=64, dtype=0)
+    for kw in (dict(head_dim=64), dict(rows=17), dict(mlp=264), dict(dtype=2)):
+        a, f = Phi3DecodeArgs(**{**good, **kw}), Phi3DecodeFp8()
+        assert lib.d3d_phi3_decode_token_fp8(C.byref(a), C.byref(f)) == -1, kw
+    a, f = Phi3DecodeArgs(**{**good, "rows": 0}), Phi3DecodeFp8()
+    assert lib.d3d_phi3_decode_token_fp8(C.byref(a), C.byref(f)) == 0

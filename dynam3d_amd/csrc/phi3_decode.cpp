@@ -67,8 +67,9 @@ extern "C" int32_t d3d_phi3_decode_token(const d3d_phi3_decode_args* a) {
     return D3D_OK;
 }
 
-// The same token with 8-bit linears: eight launches per layer (RMSNorm -> E4M3, qkv, RoPE + attention, quantise, o_proj + residual, RMSNorm -> E4M3,
-// gate_up + SwiGLU -> E4M3, down_proj + residual), of which the four products stream half the bytes of the 16-bit weights.
+// The same token with 8-bit linears: nine launches per layer (RMSNorm -> E4M3, qkv, RoPE + attention, quantise, o_proj + residual, RMSNorm -> E4M3,
+// gate_up + SwiGLU and its quantisation, down_proj + residual), of which the four products stream half the bytes of the 16-bit weights.  Eight sequences of 821 tokens,
+// 32 layers: 2.34 ms per token against 3.10 of the 16-bit path (one sequence: 2.09 against 2.59).
 extern "C" int32_t d3d_phi3_decode_token_fp8(const d3d_phi3_decode_args* a, const d3d_phi3_decode_fp8* f) {
     if (!a || !f || a->n_layers <= 0 || a->rows <= 0) return D3D_OK;
     const int32_t B = a->rows, Hd = a->hidden, H = a->heads, hd = a->head_dim, I = a->mlp, dt = a->dtype, G = 128;

@@ -413,7 +413,8 @@ k_fp8_gemm_tile(const GemmArgs a) {
 //   * Rows are permuted inside blocks of 64: row 4 f + c of a block is row f of tile c, for x and w alike.  A lane then holds 16 NEIGHBOURING columns of a row
 //     (it stores them with no trip through LDS), and the scales of its rows in four tiles are neighbours: they come by DMA too, a dword per row, are
 //     read as one 16-byte piece, and packed into a register of which the instruction picks the byte.
-//   * What bounds it: 8192^3 2.5 PFLOP/s; the matrix pipe is busy 70 % of the cycles, at 1.8 GHz (power); 16 % are waits for loads and at the barriers.  One workgroup
+//   * What bounds it: power, then waits.  8192^3 402 - 440 us, 2.5 - 2.7 PFLOP/s; the matrix pipe is busy 70 % of the cycles, at 1.8 GHz; 16 % are waits for loads and at
+//     the barriers; with a quarter of the CUs at work a K tile takes 0.97 us instead of 1.7.  One workgroup
 //     for several output tiles, loading the next one's operands while it stores, gained nothing (172.7 and 171.8 us for 6568 x 9216 x 3072).
 // DT: 0 bf16, 1 fp16, 3 E4M3 + scale (SwiGLU).  Rows of out and residual allow 16-byte accesses, columns come in eights (the host's choice of this kernel).
 // ================================================================================================================================
@@ -921,7 +922,8 @@ Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
         p.tiles_m = (M + 255) / 256;
         p.tiles_n = (ncols + (swi ? 127 : 255)) / (swi ? 128 : 256);
         p.splits = 1;
-        // (The rows of a sparse last round as a product of small tiles with K cut gained nothing: 6568 x 3072 x 8192, 252 + 60 tiles, 171.8 us against 171.0.)
+        // A sparse last round stays as it is: alone on the card its K tiles take 0.97 us, in a full round 1.7 (power and memory are shared).  6568 x 3072 x 8192, 252 + 60
+        // tiles, 171.0 us; those 60 as small tiles with K cut 171.8, as big ones with K in four slices 171.0; 2560 x 9216 x 3072 79.7 against 96.8 in slices.
         return p;
     }
     // Fewer tiles than one round of two workgroups per CU: cut K so that a round is filled, at least 4 K tiles per slice.  (us with at least 4 : 3 : 2, 77 x 1003 x 1040

@@ -413,3 +413,37 @@ def test_many_tiles_on_two_streams_and_in_a_graph():
         eager = F8.linear(z, w)
         torch.cuda.synchronize()
         assert torch.equal(out, want[j % 2]) and torch.equal(eager, want[1])
+
+
+@pytest.mark.parametrize("m,n,k", [(65600, 8, 256), (33100, 136, 272), (700, 16392, 640)])
+def test_many_tiles_hold_what_few_hold(m, n, k):
+    """A large product's rows are, bit for bit, those of products of some of them (K in one piece: both add in the same order)."""
+    x, w = operands(m, n, k, torch.float8_e8m0fnu, 2)
+    y = F8.linear(x, w)
+    for a in (0, 255, m // 2, m - 100):
+        assert torch.equal(y[a:a + 100], F8.linear(x[a:a + 100], w)), a
+    if n % 32 == 0 or n == 8:
+        x, w = operands(m // 2 + 5, 2 * 16, k, torch.float8_e8m0fnu, 2)
+        y, q = F8.linear_swiglu(x, w), F8.linear_swiglu(x, w, out_dtype=torch.float8_e4m3fn)
+        for a in (0, m // 2 - 95):
+            assert torch.equal(y[a:a + 100], F8.linear_swiglu(x[a:a + 100], w))
+            part = F8.linear_swiglu(x[a:a + 100], w, out_dtype=torch.float8_e4m3fn)
+            assert torch.equal(bits(q.data[a:a + 100]), bits(part.data)) and torch.equal(bits(q.scale[a:a + 100]), bits(part.scale))
+
+
+def test_operands_past_4_gib():
+    """x of 4.9 GB, 9.8 in 16 bits: the last rows."""
+    m, k = 600064, 8192
+    d = torch.full((m, k), 0x38, dtype=torch.uint8, device="cuda")                # 1.0
+    d[-300:] = torch.randint(0, 0x7f, (300, k), dtype=torch.uint8, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    s = torch.full((m, k // 128), 127, dtype=torch.uint8, device="cuda")
+    x = F8.Fp8(d.view(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu))
+    w = F8.quantize_weight(torch.randn(136, k, generator=gen(1)).cuda() / 90)
+    y = F8.linear(x, w)
+    ref, mag = products64(F8.Fp8(x.data[-300:].clone(), x.scale[-300:].clone()), w)
+    check(y[-300:], ref, sum_tol(mag, k, torch.bfloat16) + 2.0 ** -8 * ref.abs())
+    assert torch.equal(y[:1].expand(1000, -1), y[m - 1300:m - 300])
+    back = F8.dequantize(x[m - 300:])
+    assert torch.equal(F8.dequantize(x)[-300:], back)
+    q = F8.quantize(torch.ones(1, device="cuda", dtype=torch.bfloat16).expand(m, k))
+    assert bool((q.data[-1].float() * q.scale[-1].float().repeat_interleave(128) == 1).all())

@@ -64,6 +64,18 @@ __device__ __forceinline__ void dma_piece_once(uint32_t voff, const uint8_t* bas
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
 }
+// one scale per lane (a byte, or a float32) into the dwords behind LDS dst
+template <int KIND>
+__device__ __forceinline__ void dma_scale(uint32_t voff, const uint8_t* base, uint32_t dst) {
+    const uint32_t d = __builtin_amdgcn_readfirstlane(dst);
+    uint32_t keep;
+    if constexpr (KIND == 0)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %3\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 
 __device__ __forceinline__ v8i frag(const uint8_t* lo, const uint8_t* hi) {
@@ -219,21 +231,34 @@ k_fp8_gemm_tile(const GemmArgs a) {
         }
     };
 
-    // scales of this lane's rows: x row per i, w row (E8M0: of the lane's operand row; float32: of its 4 result columns, one block) per j
+    // Scales of this lane's rows: x row per i, w row (E8M0: of the lane's operand row; float32: of its 4 result columns, one block) per j.  They come through LDS, a
+    // DMA per wave for 64 of the 256 rows: a load per use (8 per wave, 16 rows each) kept the address pipe busier than the operands, 823 x 9216 x 3072 40 us.
+    // SwiGLU has no LDS left for them (two workgroups fill it) and loads each into its register.
+    constexpr bool LDS_SCALES = !SWI;
     const uint8_t* sxb = (const uint8_t*)a.sx + (int64_t)row0 * a.ldsx * ESZ;
     uint32_t sxo[4], swo[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        sxo[i] = (uint32_t)(min(wr * 64 + i * 16 + fi, a.M - 1 - row0) * (int)a.ldsx * ESZ);
-        swo[i] = (uint32_t)((wrow(wc * 64 + i * 16 + fi) >> 7) * (int)a.ldsw * ESZ);
-    }
-    uint32_t sx[4], sw[4], nsx[4], nsw[4];
-    auto load_scales = [&](int kt) {
-        const uint8_t *px = sxb + kt * ESZ, *pw = (const uint8_t*)a.sw + kt * ESZ;
+    if constexpr (LDS_SCALES) {
+        const int r = (wave & 1) * 64 + lane;                          // waves 0, 1: x rows, 2, 3: w rows
+        sxo[0] = (uint32_t)(wave < 2 ? min(r, a.M - 1 - row0) * (int)a.ldsx * ESZ : (wrow(r) >> 7) * (int)a.ldsw * ESZ);
+    } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            nsx[i] = KIND == 0 ? (uint32_t)px[sxo[i]] : *(const uint32_t*)(px + sxo[i]);
-            nsw[i] = KIND == 0 ? (uint32_t)pw[swo[i]] : *(const uint32_t*)(pw + swo[i]);
+            sxo[i] = (uint32_t)(min(wr * 64 + i * 16 + fi, a.M - 1 - row0) * (int)a.ldsx * ESZ);
+            swo[i] = (uint32_t)((wrow(wc * 64 + i * 16 + fi) >> 7) * (int)a.ldsw * ESZ);
+        }
+    }
+    uint32_t sx[4], sw[4], nsx[4], nsw[4];
+    auto load_scales = [&](int p) {
+        const int kt = order.tile(p);
+        const uint8_t *px = sxb + kt * ESZ, *pw = (const uint8_t*)a.sw + kt * ESZ;
+        if constexpr (LDS_SCALES) {
+            dma_scale<KIND>(sxo[0], wave < 2 ? px : pw, lds0 + 2 * STAGE + (uint32_t)(p & 1) * 1024u + (uint32_t)wave * 256u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                nsx[i] = KIND == 0 ? (uint32_t)px[sxo[i]] : *(const uint32_t*)(px + sxo[i]);
+                nsw[i] = KIND == 0 ? (uint32_t)pw[swo[i]] : *(const uint32_t*)(pw + swo[i]);
+            }
         }
     };
 
@@ -244,21 +269,28 @@ k_fp8_gemm_tile(const GemmArgs a) {
         for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
     if (order.n > 0) {
-        load_scales(order.tile(0));
+        load_scales(0);
         stage(0);
     }
     for (int p = 0; p < order.n; ++p) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();                                 // tile p has landed everywhere, tile p - 1 has been read everywhere
+        if constexpr (!LDS_SCALES) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sx[i] = nsx[i];
-            sw[i] = nsw[i];
-            asm volatile("" : "+v"(sx[i]), "+v"(sw[i]));              // the compiler's own wait for the scales belongs HERE, not behind the next DMA
+            for (int i = 0; i < 4; ++i) {
+                sx[i] = nsx[i];
+                sw[i] = nsw[i];
+                asm volatile("" : "+v"(sx[i]), "+v"(sw[i]));          // the compiler's own wait for the scales belongs HERE, not behind the next DMA
+            }
         }
         if (p + 1 < order.n) {
-            load_scales(order.tile(p + 1));
+            load_scales(p + 1);
             stage(p + 1);
+        }
+        if constexpr (LDS_SCALES) {
+            const uint32_t* ls = reinterpret_cast<const uint32_t*>(smem + 2 * STAGE + (p & 1) * 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sx[i] = ls[wr * 64 + i * 16 + fi], sw[i] = ls[128 + wc * 64 + i * 16 + fi];
         }
         const uint8_t* la = smem + (p & 1) * STAGE;
         const uint8_t* lb = la + BM * FP8_G;
@@ -953,7 +985,7 @@ int32_t allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done)
 template <int KIND, bool SWI, bool EXACT>
 int32_t launch_tile(const GemmArgs& a, hipStream_t s) {
     constexpr int BM = SWI ? 64 : 128, BN = SWI ? 256 : 128;
-    const size_t sh = 2 * (BM + BN) * FP8_G;
+    const size_t sh = 2 * (BM + BN) * FP8_G + (SWI ? 0 : 2 * 1024);
     static std::atomic<uint64_t> done{0};
     const int32_t rc = allow_lds(reinterpret_cast<const void*>(&k_fp8_gemm_tile<KIND, SWI, EXACT, BM, BN>), sh, done);
     if (rc != D3D_OK) return rc;

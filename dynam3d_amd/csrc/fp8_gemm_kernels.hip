@@ -232,7 +232,8 @@ k_fp8_gemm_tile(const GemmArgs a) {
     };
 
     // Scales of this lane's rows: x row per i, w row (E8M0: of the lane's operand row; float32: of its 4 result columns, one block) per j.  They come through LDS, a
-    // DMA per wave for 64 of the 256 rows: a load per use (8 per wave, 16 rows each) kept the address pipe busier than the operands, 823 x 9216 x 3072 40 us.
+    // DMA per wave for 64 of the 256 rows: a load per use (8 per wave, 16 rows each) kept the address pipe busier than the operands (823 x 9216 x 3072 44.5 us and
+    // 51.9 with float32 scales, now 34.4 - 37.4 and 41.3; 1024 x 3072 x 8192 72.4, now 57.2).  Loads two K tiles ahead, behind a second barrier, gained nothing (39.6).
     // SwiGLU has no LDS left for them (two workgroups fill it) and loads each into its register.
     constexpr bool LDS_SCALES = !SWI;
     const uint8_t* sxb = (const uint8_t*)a.sx + (int64_t)row0 * a.ldsx * ESZ;
@@ -948,7 +949,8 @@ Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
     p.tiles_n = (ncols + p.bn - 1) / p.bn;
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     // A round of small tiles (two workgroups per CU) takes as long as one of big tiles (one workgroup), which does twice as much.  us, small : big:
-    // 9216 x 3072, M = 256 30.5 : 39.8, 823 (504 tiles) 39.8 : 40.3, 1024 (576) 65.0 : 40.5; SwiGLU 2 x 8192 x 3072, M = 256 42.1 : 45.8, 512 (512) 50.5 : 46.6.
+    // 9216 x 3072, M = 256 27.0 : 39.8, 823 (504 tiles) 34.4 : 40.3, 1024 (576) 61.1 : 40.3; 300 x 32064 (753) 61.5 : 46.2; SwiGLU 2 x 8192 x 3072, M = 256
+    // 42.1 : 45.8, 512 (512) 50.6 : 46.0.
     if (kind == 0 && KB >= 2 && out_type != 2 && tiles >= 2 * CUS && wide && ncols % 8 == 0) {
         p.rows = -1;
         p.tiles_m = (M + 255) / 256;
@@ -959,7 +961,7 @@ Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
         return p;
     }
     // Fewer tiles than one round of two workgroups per CU: cut K so that a round is filled, at least 4 K tiles per slice.  (us with at least 4 : 3 : 2, 77 x 1003 x 1040
-    // 11.1 : 9.8 : 10.1, 100 x 3072 x 3072 15.8 : 16.5 : 20.2, 128 x 3072 x 8192 25.0 : 27.4 : 27.4, 100 x 9216 x 3072 20.9 : 22.8 : 22.9.)
+    // 10.6 : 9.5 : 9.9, 100 x 3072 x 3072 15.5 : 16.3 : 20.0, 128 x 3072 x 8192 22.7 : 26.2 : 26.4, 100 x 9216 x 3072 20.1 : 22.4 : 22.4.)
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * CUS / tiles, KB / 4));
     p.ws_bytes = p.splits > 1 ? (int64_t)p.splits * M * p.ldws * 4 : 0;
     return p;

@@ -218,8 +218,7 @@ constexpr int TM = 256, TN = 256, T_THREADS = 512;
 // that would not fill a round, each cut into `splits` K-slices so that the partial last round lasts 1/splits of a tile
 // instead of a whole one.  Every slice writes its fp32 accumulators to the workspace and leaves; k_splitk_fixup (the next launch)
 // sums the slices in slice order -- deterministic -- and runs the fused epilogue.
-// (Round 6 tried a persistent data-parallel tile walk on top of this kernel: +0.3 ... 1.1 %, but it spills -- parked with its evidence
-//  under tools/experiments/gemm_persistent_walk/.  This kernel runs at the 256-register budget with ZERO spills in the step's
+// (A persistent data-parallel tile walk on top of this kernel gained 0.3 ... 1.1 % and spilled: taken out.  This kernel runs at the 256-register budget with ZERO spills in the step's
 //  instantiations; tests/test_kernel_resources.py keeps it that way.)
 template <bool BF16, int EPI, bool KFULL, bool SPLIT, int DMAV = 0>
 __global__ void __launch_bounds__(T_THREADS, 2)

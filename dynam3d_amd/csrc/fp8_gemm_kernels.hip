@@ -100,6 +100,37 @@ __device__ __forceinline__ bf8 to_bf16(int lo, int hi) {
 }
 __device__ __forceinline__ float scale_value(uint32_t v, int kind) { return kind == 0 ? e8m0_value(v) : __uint_as_float(v); }
 
+// Two scales may multiply out of float32's range though sx sw d does not leave it (sx = 2^70, sw = 2^60, d = 2^-18; or d = 0).
+// Float32 scales in the tile kernel: their powers of two ride in the instruction as E8M0 codes (it takes any two, measured), and what multiplies the
+// sum is the product of the rests, in [1, 4).  Scalings by powers of two: the same bits as d (sx sw) where that is an ordinary number.  (A tile of 16 rows of w has
+// one scale there: the lane's operand row and its result columns share it.)
+__device__ __forceinline__ void split_scale(float s, uint32_t& code, float& rest) {
+    code = min(max((__float_as_uint(s) >> 23) & 255u, 1u), 254u);
+    rest = __builtin_ldexpf(s, 127 - (int)code);                       // (a denormal keeps its bits below 1; 0, infinity and NaN stay)
+}
+// The EXACT product has no scale operands, and in the kernel for few rows 16 rows of w may have two scales: sx * sw first while it is a normal number, else d takes the smaller one first -- that overflows only where the
+// result does, and bits it loses, below 2^-149, are bits that x or w times its scale could not hold either.
+struct ScalePair {
+    float first, second;                                               // (1, sx sw), or (the smaller, the larger)
+    __device__ __forceinline__ ScalePair(float sx, float sw) {
+        const float s = sx * sw;
+        const bool x_less = __builtin_fabsf(sx) < __builtin_fabsf(sw), plain = __builtin_fabsf(s) >= 0x1p-126f && __builtin_fabsf(s) < __builtin_inff();
+        first = plain ? 1.f : x_less ? sx : sw;
+        second = plain ? s : x_less ? sw : sx;
+    }
+    __device__ __forceinline__ float add(float d, float acc) const { return __builtin_fmaf(d * first, second, acc); }
+};
+// all 16 products of these scales are normal numbers, in every lane (NaN: whichever way, the sum becomes NaN)
+__device__ __forceinline__ bool all_plain(const float* sx, const float* sw) {
+    float hx = 0.f, hw = 0.f, lx = __builtin_inff(), lw = __builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        hx = fmaxf(hx, __builtin_fabsf(sx[i])), lx = fminf(lx, __builtin_fabsf(sx[i]));
+        hw = fmaxf(hw, __builtin_fabsf(sw[i])), lw = fminf(lw, __builtin_fabsf(sw[i]));
+    }
+    return __all(hx * hw < __builtin_inff() && lx * lw >= 0x1p-126f);
+}
+
 __device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
 
 // ---- epilogue: 4 consecutive columns n .. n + 3 of row m ------------------------------------------------------------------------------------
@@ -160,7 +191,7 @@ struct KOrder {
 //   * A K tile is one scale group: 128 B per row, the operand of ONE v_mfma_*_16x16x128.  Rows are XOR-swizzled in 16-byte chunks
 //     (chunk ^= row & 7, applied to the DMA's source address), so the two ds_read_b128 of a fragment are conflict-free.
 //   * w is the first operand: a lane owns 4 consecutive columns of one row of the result.
-//   * E8M0: the scales ride in the instruction.  float32 scales, and EXACT: each K tile's product is multiplied by sx * sw and added.
+//   * E8M0: the scales ride in the instruction.  float32 scales, and EXACT: each K tile's product is multiplied by sx * sw and added (split_scale, ScalePair).
 // SwiGLU: the tile holds BN / 2 columns of the result; its w rows alternate 16 gate and 16 up rows, so that one lane holds both.
 // ================================================================================================================================
 template <int KIND, bool SWI, bool EXACT, int BM, int BN>
@@ -273,7 +304,10 @@ k_fp8_gemm_tile(const GemmArgs a) {
         load_scales(0);
         stage(0);
     }
-    for (int p = 0; p < order.n; ++p) {
+    constexpr bool CARE = EXACT || KIND == 1;                         // scales as numbers: their products may not be
+    float fx[4], fw[4];
+    v8i af[4], bf[4];                                                 // (EXACT reads its fragments by halves)
+    auto arrive = [&](int p) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();                                 // tile p has landed everywhere, tile p - 1 has been read everywhere
         if constexpr (!LDS_SCALES) {
@@ -293,9 +327,27 @@ k_fp8_gemm_tile(const GemmArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) sx[i] = ls[wr * 64 + i * 16 + fi], sw[i] = ls[128 + wc * 64 + i * 16 + fi];
         }
-        const uint8_t* la = smem + (p & 1) * STAGE;
-        const uint8_t* lb = la + BM * FP8_G;
+    };
+    auto fetch = [&](int p) {
+        if constexpr (!EXACT) {
+            const uint8_t* la = smem + (p & 1) * STAGE;
+            const uint8_t* lb = la + BM * FP8_G;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int rb = wc * 64 + i * 16 + fi, ra = wr * 64 + i * 16 + fi, s = fi & 7;
+                bf[i] = frag(lb + rb * FP8_G + ((fg ^ s) << 4), lb + rb * FP8_G + (((fg + 4) ^ s) << 4));
+                af[i] = frag(la + ra * FP8_G + ((fg ^ s) << 4), la + ra * FP8_G + (((fg + 4) ^ s) << 4));
+            }
+        }
+        if constexpr (CARE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fx[i] = scale_value(sx[i], KIND), fw[i] = scale_value(sw[i], KIND);
+        }
+    };
+    auto multiply = [&](int p, auto plain) {                          // plain: sx * sw is a normal number for all pairs of the wave
         if constexpr (EXACT) {
+            const uint8_t* la = smem + (p & 1) * STAGE;
+            const uint8_t* lb = la + BM * FP8_G;
 #pragma unroll
             for (int jh = 0; jh < 4; jh += 2) {                       // two of the wave's four column tiles at a time: the sums of a K tile are 32 registers
                 v4f d[4][2];
@@ -325,18 +377,16 @@ k_fp8_gemm_tile(const GemmArgs a) {
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float s = scale_value(sx[i], KIND) * scale_value(sw[jh + j], KIND);
+                        const ScalePair s(fx[i], fw[jh + j]);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[i][jh + j][r] = __builtin_fmaf(d[i][j][r], s, acc[i][jh + j][r]);
+                        for (int r = 0; r < 4; ++r)
+                            acc[i][jh + j][r] = plain ? __builtin_fmaf(d[i][j][r], fx[i] * fw[jh + j], acc[i][jh + j][r]) : s.add(d[i][j][r], acc[i][jh + j][r]);
                     }
             }
         } else {
-            v8i af[4], bf[4];
+            if constexpr (KIND == 1 && !plain) {                      // the codes to sx, sw, the rests to fx, fw
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int rb = wc * 64 + i * 16 + fi, ra = wr * 64 + i * 16 + fi, s = fi & 7;
-                bf[i] = frag(lb + rb * FP8_G + ((fg ^ s) << 4), lb + rb * FP8_G + (((fg + 4) ^ s) << 4));
-                af[i] = frag(la + ra * FP8_G + ((fg ^ s) << 4), la + ra * FP8_G + (((fg + 4) ^ s) << 4));
+                for (int i = 0; i < 4; ++i) split_scale(fx[i], sx[i], fx[i]), split_scale(fw[i], sw[i], fw[i]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -345,14 +395,40 @@ k_fp8_gemm_tile(const GemmArgs a) {
                     if constexpr (KIND == 0) {
                         acc[i][j] = mma_scaled(bf[j], af[i], acc[i][j], sw[j], sx[i]);
                     } else {
-                        const v4f d = mma_plain(bf[j], af[i], v4f{0.f, 0.f, 0.f, 0.f});
-                        const float s = __uint_as_float(sx[i]) * __uint_as_float(sw[j]);
+                        const v4f zero = v4f{0.f, 0.f, 0.f, 0.f}, d = plain ? mma_plain(bf[j], af[i], zero) : mma_scaled(bf[j], af[i], zero, sw[j], sx[i]);
+                        const float s = fx[i] * fw[j];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(d[r], s, acc[i][j][r]);
                     }
                 }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    // Products of scales that are not plain are rare (zeros beside small weights make them, 2^-126 * sw): the first one sends the wave to a second loop that takes care of
+    // them.  Both loops meet the workgroup's other waves at one barrier per K tile.  (6568 x 3072 x 8192, float32 scales: 207 us, without the question 197, in the careful
+    // form for every K tile 216; both forms in one loop spilled.)
+    int p = 0;
+    if constexpr (CARE) {
+        bool plain = true;
+        while (p < order.n) {
+            arrive(p);
+            fetch(p);
+            plain = all_plain(fx, fw);
+            if (!plain) break;
+            multiply(p++, std::true_type{});
+        }
+        while (!plain) {
+            fetch(p);
+            multiply(p++, std::false_type{});
+            if (p == order.n) break;
+            arrive(p);
+        }
+    } else {
+        for (; p < order.n; ++p) {
+            arrive(p);
+            fetch(p);
+            multiply(p, std::true_type{});
+        }
     }
 
     // ---- epilogue: lane holds row row0 + wr * 64 + i * 16 + fi, operand columns wc * 64 + j * 16 + fg * 4 .. + 3
@@ -803,9 +879,9 @@ k_fp8_gemm_rows(const GemmArgs a, int R /* <= 16 NJ, a multiple of 4 */, int nb 
                             acc[i * NW + t] = mma_scaled(w, xv, acc[i * NW + t], sw[t], sx[i]);
                         } else {
                             const v4f d = mma_plain(w, xv, v4f{0.f, 0.f, 0.f, 0.f});
-                            const float s = __uint_as_float(sx[i]) * __uint_as_float(sw[t]);
+                            const ScalePair s(__uint_as_float(sx[i]), __uint_as_float(sw[t]));
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) acc[i * NW + t][r] = __builtin_fmaf(d[r], s, acc[i * NW + t][r]);
+                            for (int r = 0; r < 4; ++r) acc[i * NW + t][r] = s.add(d[r], acc[i * NW + t][r]);
                         }
                     }
                 }
@@ -832,9 +908,9 @@ k_fp8_gemm_rows(const GemmArgs a, int R /* <= 16 NJ, a multiple of 4 */, int nb 
                     }
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        const float s = scale_value(sx[i], KIND) * scale_value(sw[t], KIND);
+                        const ScalePair s(scale_value(sx[i], KIND), scale_value(sw[t], KIND));
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[i * NW + t][r] = __builtin_fmaf(d[i][r], s, acc[i * NW + t][r]);
+                        for (int r = 0; r < 4; ++r) acc[i * NW + t][r] = s.add(d[i][r], acc[i * NW + t][r]);
                     }
                 }
             }

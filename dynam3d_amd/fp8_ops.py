@@ -33,6 +33,7 @@ E4M3_MAX = 448.0
 _LEAST = 2.0 ** -126
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, E4M3: 3}
 _KIND = {E8M0: 0, torch.float32: 1}
+_MOST = 2 ** 31 - 1                                    # rows and columns are 32-bit numbers in the C entry points (ctypes would cut longer ones off without a word)
 
 
 class _GemmArgs(C.Structure):
@@ -99,6 +100,11 @@ def _unit_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
+def _check_sizes(name, *sizes):
+    if max(sizes) > _MOST:
+        raise ValueError(f"fp8_ops.{name}: {max(sizes)} rows or columns: at most 2^31 - 1")
+
+
 def _check_input(name, x, scale_dtype):
     if x.dim() != 2 or x.dtype not in _DT or x.dtype == E4M3:
         raise TypeError(f"fp8_ops.{name}: a matrix (rows, K) of bfloat16, float16 or float32, not {tuple(x.shape)} {x.dtype}")
@@ -106,6 +112,7 @@ def _check_input(name, x, scale_dtype):
         raise TypeError(f"fp8_ops.{name}: scale_dtype is float8_e8m0fnu or float32, not {scale_dtype}")
     if x.shape[1] == 0 or x.shape[1] % 16:
         raise ValueError(f"fp8_ops.{name}: K = {x.shape[1]} has to be a positive multiple of 16 (the operand of the product is read in 16-byte pieces)")
+    _check_sizes(name, *x.shape)
 
 
 def _same_device(name, first, *others):
@@ -178,6 +185,7 @@ def dequantize(q: Fp8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values q.data * q.scale, rounded once to `dtype` (exact in bf16 for power-of-two scales)."""
     if dtype not in _DT or dtype == E4M3:
         raise TypeError(f"fp8_ops.dequantize: to bfloat16, float16 or float32, not {dtype}")
+    _check_sizes("dequantize", *q.shape)
     if not q.data.is_cuda:
         return _cpu_values(q).to(dtype)
     if q.shape[1] % 16:
@@ -240,6 +248,7 @@ def _workspace_bytes(m, n, k, swiglu, out_type, kind):
 
 def workspace_bytes(m: int, n: int, k: int, swiglu: bool = False, out_dtype: torch.dtype = torch.bfloat16, scale_dtype: torch.dtype = E8M0) -> int:
     """Scratch that a C caller of `d3d_fp8_gemm` has to bring for a product of x (m, k) with w (n, k)."""
+    _check_sizes("workspace_bytes", m, n, k)
     return _workspace_bytes(m, n, k, int(swiglu), _DT[out_dtype], _KIND[scale_dtype])
 
 
@@ -275,6 +284,7 @@ def _check_operands(name, x, w):
         raise TypeError(f"fp8_ops.{name}: x from quantize() / rms_norm() (one scale per row), w from quantize_weight() (one per 128 x 128 block)")
     if x.data.shape[1] != w.data.shape[1] or x.data.shape[1] == 0 or x.data.shape[1] % 16:
         raise ValueError(f"fp8_ops.{name}: x {tuple(x.shape)} and w {tuple(w.shape)}: the same K, a positive multiple of 16")
+    _check_sizes(name, *x.shape, *w.shape)
     if x.scale.dtype != w.scale.dtype:
         raise TypeError(f"fp8_ops.{name}: scales of x {x.scale.dtype} and of w {w.scale.dtype}: one type for both")
     if x.data.device != w.data.device:

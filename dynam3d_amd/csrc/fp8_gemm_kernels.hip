@@ -1005,10 +1005,10 @@ struct Plan {
     int64_t ldws, ws_bytes;
 };
 
-// wide: rows of out and residual start on 16 bytes
-Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
+// wide: rows of out and residual start on 16 bytes.  (64-bit sizes: M, N up to 2^31 - 1 are rounded up to tiles here)
+Plan plan_of(int64_t M, int64_t N, int64_t K, bool swi, int out_type, int kind, bool wide) {
     Plan p{};
-    const int KB = (K + FP8_G - 1) / FP8_G, ncols = swi ? N / 2 : N;
+    const int64_t KB = (K + FP8_G - 1) / FP8_G, ncols = swi ? N / 2 : N;
     p.ldws = swi ? 2 * ((ncols + 7) / 8 * 8) : (ncols + 7) / 8 * 8;
     // Few rows: the weights stream once (device time at K = 3072, N = 9216, us, against the tile kernel: M = 17 9.4 : 15.1, 32 10.4 : 16.0, 64 13.3 : 18.0;
     // K = 8192, N = 3072: 32 12.3 : 18.7, 64 16.5 : 20.1).  Behind 32 rows x is most of what a workgroup of a wide product reads: N = 32064 at 64 rows
@@ -1016,21 +1016,21 @@ Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
     if (M <= 32 || (M <= 64 && ncols <= 64 * CUS)) {
         p.rows = M <= 16 ? 1 : M <= 32 ? 2 : 4;
         p.splits = 1;
-        p.ws_bytes = out_type == 3 ? (int64_t)M * p.ldws * 4 : 0;
+        p.ws_bytes = out_type == 3 ? M * p.ldws * 4 : 0;
         return p;
     }
     p.bm = swi ? 64 : 128;
     p.bn = 128;                                                        // columns of the result per tile (SwiGLU: 256 rows of w)
-    p.tiles_m = (M + p.bm - 1) / p.bm;
-    p.tiles_n = (ncols + p.bn - 1) / p.bn;
+    p.tiles_m = (int)((M + p.bm - 1) / p.bm);
+    p.tiles_n = (int)((ncols + p.bn - 1) / p.bn);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     // A round of small tiles (two workgroups per CU) takes as long as one of big tiles (one workgroup), which does twice as much.  us, small : big:
     // 9216 x 3072, M = 256 27.0 : 39.8, 823 (504 tiles) 34.4 : 40.3, 1024 (576) 61.1 : 40.3; 300 x 32064 (753) 61.5 : 46.2; SwiGLU 2 x 8192 x 3072, M = 256
     // 42.1 : 45.8, 512 (512) 50.6 : 46.0.
     if (kind == 0 && KB >= 2 && out_type != 2 && tiles >= 2 * CUS && wide && ncols % 8 == 0) {
         p.rows = -1;
-        p.tiles_m = (M + 255) / 256;
-        p.tiles_n = (ncols + (swi ? 127 : 255)) / (swi ? 128 : 256);
+        p.tiles_m = (int)((M + 255) / 256);
+        p.tiles_n = (int)((ncols + (swi ? 127 : 255)) / (swi ? 128 : 256));
         p.splits = 1;
         // A sparse last round stays as it is: alone on the card its K tiles take 0.97 us, in a full round 1.7 (power and memory are shared).  6568 x 3072 x 8192, 252 + 60
         // tiles, 171.0 us; those 60 as small tiles with K cut 171.8, as big ones with K in four slices 171.0; 2560 x 9216 x 3072 79.7 against 96.8 in slices.
@@ -1039,7 +1039,7 @@ Plan plan_of(int M, int N, int K, bool swi, int out_type, int kind, bool wide) {
     // Fewer tiles than one round of two workgroups per CU: cut K so that a round is filled, at least 4 K tiles per slice.  (us with at least 4 : 3 : 2, 77 x 1003 x 1040
     // 10.6 : 9.5 : 9.9, 100 x 3072 x 3072 15.5 : 16.3 : 20.0, 128 x 3072 x 8192 22.7 : 26.2 : 26.4, 100 x 9216 x 3072 20.1 : 22.4 : 22.4.)
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * CUS / tiles, KB / 4));
-    p.ws_bytes = p.splits > 1 ? (int64_t)p.splits * M * p.ldws * 4 : 0;
+    p.ws_bytes = p.splits > 1 ? p.splits * M * p.ldws * 4 : 0;
     return p;
 }
 
@@ -1074,12 +1074,13 @@ int32_t launch_tile(const GemmArgs& a, hipStream_t s) {
 template <int KIND, bool SWI, bool EXACT, int MT, int NJ>
 int32_t launch_rows_of(const GemmArgs& a, int R, hipStream_t s) {
     constexpr int NW = NJ * (SWI ? 2 : 1), T = MT * NW, U = 4 / MT, WAVES = SWI || MT == 4 ? 8 : 16, SLOT = (NW + MT) * 2048, LDS = 160 * 1024;
-    const int grid = ((SWI ? a.I : a.N) + R - 1) / R;
+    const int64_t grid = ((int64_t)(SWI ? a.I : a.N) + R - 1) / R;
     const int per = (a.KB + WAVES - 1) / WAVES, nw = (a.KB + per - 1) / per;                    // K blocks of a wave; the waves that takes
     // more workgroups than CUs: two of them per CU, so that one loads while the other adds up (16384 x 3072 at 8 rows: 12.2 us; one, with twice
     // the blocks in flight: 14.2)
     const int nb = std::min({U, per, std::max(1, (grid > CUS ? LDS / 2 : LDS) / (nw * SLOT))});
     const size_t sh = (size_t)nw * std::max(nb * SLOT, T * 1024);
+    if (grid * nw * 64 >= (int64_t)1 << 32) return bad("d3d_fp8_gemm: too many columns for one launch");
     static_assert(WAVES * (SLOT > T * 1024 ? SLOT : T * 1024) <= LDS, "one block per wave fits");
     static std::atomic<uint64_t> done{0};
     const int32_t rc = allow_lds(reinterpret_cast<const void*>(&k_fp8_gemm_rows<KIND, SWI, EXACT, MT, NJ, U, WAVES>), LDS, done);
@@ -1091,8 +1092,8 @@ template <int KIND, bool SWI, bool EXACT, int MT>
 int32_t launch_rows(const GemmArgs& a, hipStream_t s) {
     // R: one workgroup per CU up to 48 rows (SwiGLU: 16), else a whole number of them of up to 32
     constexpr int MOST = SWI ? 16 : 48, MANY = SWI ? 16 : 32;
-    const int ncols = SWI ? a.I : a.N, per_cu = ncols <= CUS * MOST ? 1 : (ncols + CUS * MANY - 1) / (CUS * MANY);
-    const int R = std::max(8, ((ncols + CUS * per_cu - 1) / (CUS * per_cu) + 3) / 4 * 4);
+    const int64_t ncols = SWI ? a.I : a.N, per_cu = ncols <= CUS * MOST ? 1 : (ncols + CUS * MANY - 1) / (CUS * MANY);
+    const int R = std::max(8, (int)((ncols + CUS * per_cu - 1) / (CUS * per_cu) + 3) / 4 * 4);
     if constexpr (MOST > 16) {
         if (R > 32) return launch_rows_of<KIND, SWI, EXACT, MT, 3>(a, R, s);
         if (R > 16) return launch_rows_of<KIND, SWI, EXACT, MT, 2>(a, R, s);
@@ -1151,11 +1152,14 @@ int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
     if (((uintptr_t)g->x & 15) || ((uintptr_t)g->w & 15) || g->ldx % 16 || g->ldw % 16 || g->ldx < 0 || g->ldw < 0)
         return bad("d3d_fp8_gemm: rows of x and w must start on 16 bytes");
     if (g->out_type == 3 && (((uintptr_t)g->out & 15) || g->ldo % 16)) return bad("d3d_fp8_gemm: rows of a quantised result must start on 16 bytes");
+    if (g->K >= 1 << 24) return bad("d3d_fp8_gemm: K of 2^24 and more");
     if (g->ldx >= (int64_t)1 << 24 || g->ldw >= (int64_t)1 << 24) return bad("d3d_fp8_gemm: rows further than 16 MiB apart");
     if (g->ldsx < 0 || g->ldsw < 0 || g->ldsx >= 1 << 20 || (int64_t)(g->N / FP8_G + 1) * g->ldsw >= 1 << 29) return bad("d3d_fp8_gemm: scale rows too far apart");
     if (swi && (int64_t)g->N * g->ldw >= (int64_t)1 << 32) return bad("d3d_fp8_gemm: SwiGLU weights of 4 GiB and more");
     const bool wide = ((uintptr_t)g->out & 15) == 0 && g->ldo % 8 == 0 && g->ldo < 1 << 22 && g->ldr < 1 << 22 && (!g->residual || (((uintptr_t)g->residual & 15) == 0 && g->ldr % 8 == 0)) && ((uintptr_t)g->bias & 15) == 0;
     const Plan p = plan_of(g->M, g->N, g->K, swi, g->out_type, g->scale_kind, wide);
+    const int64_t c8 = ((int64_t)ncols + 127) / 128 * 16;              // threads per row of k_fp8_gemm_finish
+    if (p.ws_bytes && g->M * c8 >= ((int64_t)1 << 32) - 256) return bad("d3d_fp8_gemm: too many columns for one launch");
     if (p.rows <= 0 && (int64_t)p.tiles_m * p.tiles_n * p.splits >= (int64_t)1 << 24) return bad("d3d_fp8_gemm: too many tiles for one launch");
     if (p.ws_bytes > g->workspace_bytes || (p.ws_bytes && (!g->workspace || ((uintptr_t)g->workspace & 15))))
         return bad("d3d_fp8_gemm: workspace smaller than d3d_fp8_gemm_workspace() or not on 16 bytes");
@@ -1173,9 +1177,8 @@ int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
     const int32_t rc = swi ? (g->scale_kind == 0 ? launch<0, true>(a, p.rows, s) : launch<1, true>(a, p.rows, s))
                            : (g->scale_kind == 0 ? launch<0, false>(a, p.rows, s) : launch<1, false>(a, p.rows, s));
     if (rc != D3D_OK || !p.ws_bytes) return rc;
-    const int c8 = (ncols + 127) / 128 * 16;
-    const int64_t nb = ((int64_t)a.M * c8 + 255) / 256;
-    hipLaunchKernelGGL(k_fp8_gemm_finish, dim3((uint32_t)nb), dim3(256), 0, s, a, swi ? 1 : 0, c8, g->scale_kind);
+    const int64_t nb = (a.M * c8 + 255) / 256;
+    hipLaunchKernelGGL(k_fp8_gemm_finish, dim3((uint32_t)nb), dim3(256), 0, s, a, swi ? 1 : 0, (int)c8, g->scale_kind);
     D3D_LAUNCH_CHECK();
 }
 

@@ -210,7 +210,7 @@ int32_t d3d_fp8_quantize(const void* x, void* q, void* scale, int32_t rows, int3
     if (rows < 0 || K < 0 || K % 16 || dtype < 0 || dtype > 2 || scale_kind < 0 || scale_kind > 1) return bad("d3d_fp8_quantize: bad sizes (K must be a multiple of 16) or types");
     if (rows == 0 || K == 0) return D3D_OK;
     if (!x || !q || !scale || !aligned(x, ldx, elem_bytes(dtype)) || !aligned(q, ldq, 1)) return bad("d3d_fp8_quantize: rows must start on 16 bytes");
-    const int KB = (K + FP8_G - 1) / FP8_G;
+    const int KB = (int)(((int64_t)K + FP8_G - 1) / FP8_G);            // (K up to 2^31 - 16)
     const int64_t nb = ((int64_t)rows * KB + 15) / 16;
     if (!blocks_ok(nb)) return bad("d3d_fp8_quantize: too many groups for one launch");
 #define CALL(DT) \
@@ -225,7 +225,7 @@ int32_t d3d_fp8_quantize_weight(const void* w, void* q, void* scale, int32_t row
     if (rows < 0 || K < 0 || K % 16 || dtype < 0 || dtype > 2 || scale_kind < 0 || scale_kind > 1) return bad("d3d_fp8_quantize_weight: bad sizes (K must be a multiple of 16) or types");
     if (rows == 0 || K == 0) return D3D_OK;
     if (!w || !q || !scale || !aligned(w, ldw, elem_bytes(dtype)) || !aligned(q, ldq, 1)) return bad("d3d_fp8_quantize_weight: rows must start on 16 bytes");
-    const int KB = (K + FP8_G - 1) / FP8_G, NB = (rows + FP8_G - 1) / FP8_G;
+    const int KB = (int)(((int64_t)K + FP8_G - 1) / FP8_G), NB = (int)(((int64_t)rows + FP8_G - 1) / FP8_G);
     if (NB > 65535) return bad("d3d_fp8_quantize_weight: more than 65535 blocks of rows");
 #define CALL(DT) \
     hipLaunchKernelGGL((k_fp8_quant_block<DT>), dim3(KB, NB), dim3(256), 0, (hipStream_t)stream, w, (uint8_t*)q, scale, rows, K, ldw, ldq, lds, scale_kind)

@@ -37,3 +37,20 @@ def test_rows_past_32_bits_are_refused(rows):
               lambda: F8.workspace_bytes(rows, 64, 256), lambda: F8.workspace_bytes(64, rows, 256)):
         with pytest.raises(ValueError, match="at most 2\\^31 - 1"):
             f()
+
+
+def test_sizes_near_2_to_the_31():
+    lib, most, k = _lib.load(), 2 ** 31 - 1, 2 ** 31 - 16
+    assert lib.d3d_fp8_quantize(P, P, P, most, k, k, k, 1 << 24, 0, 0, None) == -1
+    assert lib.d3d_fp8_quantize_weight(P, P, P, most, 64, 64, 64, 1, 0, 0, None) == -1
+    assert lib.d3d_fp8_quantize_weight(P, P, P, most - 126, 64, 64, 64, 1, 0, 0, None) == -1
+    for kw in (dict(M=most, scale_kind=1, N=8, ldo=8), dict(M=most - 126, out_type=2, N=8, ldo=8), dict(M=most, N=most, ldo=most), dict(M=most - 100, N=1 << 20, ldo=1 << 20),
+               dict(M=1, N=most, K=4096, ldx=4096, ldw=0, ldsw=0), dict(M=32, N=k - 16, ldw=0, ldsw=0, swiglu=1, out_type=3, ldo=1 << 30, ldos=1 << 23)):
+        assert refused(b"d3d_fp8_gemm: too many", **kw), (kw, lib.d3d_last_error())
+    for kw in (dict(K=1 << 24), dict(K=k)):
+        assert refused(b"d3d_fp8_gemm: K of", ldx=0, ldw=0, ldsx=0, ldsw=0, **kw)
+    # 2^31 - 1 rows are whole tiles of 128 and of 256: neither kernel asks for scratch, nor for a number of tiles that wrapped
+    for m in (most, most - 120, most - 254):
+        for out, kind in ((0, 0), (0, 1), (2, 0)):
+            assert F8._workspace_bytes(m, 8, 256, 0, out, kind) == 0
+    assert F8._workspace_bytes(32, 2 ** 30, 256, 1, 3, 0) == 32 * 2 ** 30 * 4

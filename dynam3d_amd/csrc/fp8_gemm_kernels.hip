@@ -1156,6 +1156,9 @@ int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* g) {
     if (g->ldx >= (int64_t)1 << 24 || g->ldw >= (int64_t)1 << 24) return bad("d3d_fp8_gemm: rows further than 16 MiB apart");
     if (g->ldsx < 0 || g->ldsw < 0 || g->ldsx >= 1 << 20 || (int64_t)(g->N / FP8_G + 1) * g->ldsw >= 1 << 29) return bad("d3d_fp8_gemm: scale rows too far apart");
     if (swi && (int64_t)g->N * g->ldw >= (int64_t)1 << 32) return bad("d3d_fp8_gemm: SwiGLU weights of 4 GiB and more");
+    if (g->ldr < 0) return bad("d3d_fp8_gemm: residual rows in descending order");
+    if (g->ldo < 0 || (g->M > 1 && (g->ldo < ncols || (g->out_type == 3 && g->ldos < (ncols + FP8_G - 1) / FP8_G))))
+        return bad("d3d_fp8_gemm: rows of the result would lie over one another");
     const bool wide = ((uintptr_t)g->out & 15) == 0 && g->ldo % 8 == 0 && g->ldo < 1 << 22 && g->ldr < 1 << 22 && (!g->residual || (((uintptr_t)g->residual & 15) == 0 && g->ldr % 8 == 0)) && ((uintptr_t)g->bias & 15) == 0;
     const Plan p = plan_of(g->M, g->N, g->K, swi, g->out_type, g->scale_kind, wide);
     const int64_t c8 = ((int64_t)ncols + 127) / 128 * 16;              // threads per row of k_fp8_gemm_finish

@@ -647,7 +647,8 @@ int32_t d3d_fp8_rms_norm(const void* x, const void* residual, const float* w, vo
  * residual have that type; residual may be out).  swiglu: w = [gate (N/2 rows); up (N/2 rows)], y = up * silu(gate), (M, N/2), no bias or
  * residual; out_type 3 = E4M3 + out_scale (M, ceil(N/2/128)) of the same scale_kind.  Both scales are of scale_kind, any
  * finite values: they may multiply out of float32's range where the result does not.  `workspace`: d3d_fp8_gemm_workspace() bytes of device
- * memory on 16 bytes, used until the call's work on `stream` has ended (0: none needed). */
+ * memory on 16 bytes, used until the call's work on `stream` has ended (0: none needed).  K < 2^24; rows of x and w less than 2^24 apart; ldr >= 0
+ * (0: one row for all); rows of out and out_scale do not overlap. */
 typedef struct d3d_fp8_gemm_args {
     const void *x, *sx, *w, *sw, *bias, *residual;
     void *out, *out_scale, *workspace;

@@ -54,3 +54,11 @@ def test_sizes_near_2_to_the_31():
         for out, kind in ((0, 0), (0, 1), (2, 0)):
             assert F8._workspace_bytes(m, 8, 256, 0, out, kind) == 0
     assert F8._workspace_bytes(32, 2 ** 30, 256, 1, 3, 0) == 32 * 2 ** 30 * 4
+
+
+def test_strides_that_the_epilogues_do_not_take():
+    """Large products address residual and result rows by unsigned 32-bit offsets from a tile's first row."""
+    large = dict(M=4096, N=8192, ldo=8192, ldr=8192, residual=P)
+    for kw in (dict(ldo=-64), dict(ldo=63), dict(ldo=0), dict(ldr=-64, residual=P), dict(large, ldr=-8192), dict(large, ldo=-8192), dict(large, ldo=8184),
+               dict(swiglu=1, out_type=3, ldo=16), dict(swiglu=1, N=512, out_type=3, ldo=256, ldos=1), dict(swiglu=1, N=512, out_type=3, ldo=256, ldos=-2)):
+        assert refused(b"rows", **kw), (kw, _lib.load().d3d_last_error())

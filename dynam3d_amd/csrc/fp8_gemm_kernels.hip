@@ -131,7 +131,23 @@ __device__ __forceinline__ bool all_plain(const float* sx, const float* sw) {
     return __all(hx * hw < __builtin_inff() && lx * lw >= 0x1p-126f);
 }
 
-__device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
+// __expf rounds x log2(e) before the power: its error grows to |x| 2^-24 (5e-6 at 88), far inside the rounding of an 8- or 16-bit result.  A float32 result (FULL) gets
+// e^x = 2^n 2^f with f = x log2(e) - n from two fused operations (log2(e) in two parts): within 2^-22 for every x, of a negative argument so that it cannot overflow.
+// (expf would do, but this file is compiled with -ffp-contract=fast, which fuses expf's own reduction apart: 2.6e-6 at 80.)
+__device__ __forceinline__ float exp_below_0(float x) {
+    x = fmaxf(x, -150.f);                                              // (2^-216: 0)
+    const float n = __builtin_rintf(x * 0x1.715476p+0f), f = __builtin_fmaf(x, 0x1.4ae0cp-26f, __builtin_fmaf(x, 0x1.715476p+0f, -n));
+    return __builtin_ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+}
+template <bool FULL>
+__device__ __forceinline__ float silu(float x) {
+    if constexpr (FULL) {
+        const float e = exp_below_0(-__builtin_fabsf(x));
+        return x * ((x < 0.f ? e : 1.f) / (1.f + e));
+    } else {
+        return x / (1.f + __expf(-x));
+    }
+}
 
 // ---- epilogue: 4 consecutive columns n .. n + 3 of row m ------------------------------------------------------------------------------------
 template <int DT>
@@ -466,7 +482,7 @@ k_fp8_gemm_tile(const GemmArgs a) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[i][j * 4 + r] = acc[i][2 * j + 1][r] * silu(acc[i][2 * j][r]);
+                for (int r = 0; r < 4; ++r) v[i][j * 4 + r] = acc[i][2 * j + 1][r] * silu<EXACT>(acc[i][2 * j][r]);
         if (a.out_type != 3) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -704,7 +720,7 @@ k_fp8_gemm_big(const GemmArgs a) {
                 float y = 0.f;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    const float v = acc[i][h * 4 + 2 + (c & 1)][c >> 1] * silu(acc[i][h * 4 + (c & 1)][c >> 1]);
+                    const float v = acc[i][h * 4 + 2 + (c & 1)][c >> 1] * silu<false>(acc[i][h * 4 + (c & 1)][c >> 1]);
                     acc[i][h * 4 + (c & 1)][c >> 1] = v;
                     y = fmaxf(y, fp8_finite_abs(v));
                 }
@@ -769,7 +785,7 @@ k_fp8_gemm_big(const GemmArgs a) {
                 float v[NC];
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
-                    if constexpr (SWI) v[c] = acc[i][h * 4 + 2 + (c & 1)][c >> 1] * silu(acc[i][h * 4 + (c & 1)][c >> 1]);
+                    if constexpr (SWI) v[c] = acc[i][h * 4 + 2 + (c & 1)][c >> 1] * silu<false>(acc[i][h * 4 + (c & 1)][c >> 1]);
                     else v[c] = acc[i][h * 4 + (c & 3)][c >> 2] + half(bias[c >> 3], c & 7) + half(t[i][c >> 3], c & 7);
                 }
                 uint8_t* o = obase + ((uint32_t)row_of(i) * (uint32_t)a.ldo * 2u + on);
@@ -941,7 +957,7 @@ k_fp8_gemm_rows(const GemmArgs a, int R /* <= 16 NJ, a multiple of 4 */, int nb 
                 continue;
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[0][r] = v[1][r] * silu(v[0][r]);
+            for (int r = 0; r < 4; ++r) v[0][r] = v[1][r] * silu<EXACT>(v[0][r]);
         }
         finish4(a, v[0], m, n, n0 + rows);
     }
@@ -971,7 +987,7 @@ k_fp8_gemm_finish(const GemmArgs a, int swi, int c8 /* threads per row: a multip
         }
         if (swi) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = u[i] * silu(v[i]);
+            for (int i = 0; i < 8; ++i) v[i] = u[i] * (a.out_type == 2 ? silu<true>(v[i]) : silu<false>(v[i]));
         }
         if (a.out_type != 3) {
             finish4(a, v, m, n, ncols);

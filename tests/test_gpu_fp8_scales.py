@@ -95,3 +95,23 @@ def test_rows_of_zeros_change_nothing_beside_them(m, kind, out):
             ref, size = d @ v.t(), d.abs() @ v.abs().t()
             tol = (2 * (512 + 4) * 2.0 ** -24 + (0.0 if out == F32 else 7 * 2.0 ** -13)) * size + torch.finfo(out).eps / 2 * ref.abs()
             assert bool(((y.double() - ref).abs() <= tol)[none.cuda()].all())
+
+
+@pytest.mark.parametrize("kind", [E8M0, F32])
+@pytest.mark.parametrize("k", [16, 1040])
+@pytest.mark.parametrize("m", [1, 20, 40, 100, 300])
+def test_silu_of_float32_results(m, k, kind):
+    """Gates from -80 to 80 and ups of 1, both exact sums: what is left are the exponential (1 ulp: 2^-23), the sum, the quotient and two products behind it (2^-24
+    each) -- 2^-21 relative.  Few rows, tiles, and K in slices joined by another kernel (100 rows, K = 1040)."""
+    gates = torch.arange(-320, 321).double() / 4
+    i = 656
+    w = torch.zeros(2 * i, k)
+    for n, g in enumerate(gates.tolist()):
+        for bit in range(10):                                                       # one power of two per column
+            w[n, bit] = (1.0 if g >= 0 else -1.0) * 2.0 ** (bit - 2) if int(abs(g) * 4) >> bit & 1 else 0.0
+    w[i:, 12] = 1.0
+    one = lambda r, rows: torch.ones((r + rows - 1) // rows, (k + 127) // 128).to(kind).cuda()
+    x = F8.Fp8(torch.ones(m, k).to(E4M3).cuda(), one(m, 1))
+    y = F8.linear_swiglu(x, F8.Fp8(w.to(E4M3).cuda(), one(2 * i, 128), 128), out_dtype=F32)[:, :641].double().cpu()
+    want = gates / (1 + torch.exp(-gates))
+    assert bool(((y - want).abs() <= 2.0 ** -21 * want.abs()).all()), float(((y - want).abs() / want.abs().clamp_min(1e-300)).max())

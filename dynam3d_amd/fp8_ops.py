@@ -13,6 +13,12 @@ applies it for free --, or torch.float32: s = max(amax / 448, 2^-126).  amax run
 nearest even, and a member that is not finite becomes E4M3's NaN: it poisons its own row of a product, never its neighbours.  A product takes
 two operands of the same scale type.
 
+Products.  gfx950's 8-bit matrix instruction aligns 8 neighbouring products to the largest of them and drops what lies 13 bits below it: a sum is off by at most
+7 * 2^-13 sum |x w|, ~2^-14 of a result of random signs, before its one rounding -- inside half a step of bf16 (2^-9) and of fp16 (2^-12) unless most of the
+sum cancels; a result that is quantised again lands on the other E4M3 neighbour once in ~650 members.  `exact=True` takes the bf16 instruction instead, whose
+products of E4M3 values are exact (float32 sums), for 1 to 3 times the time; float32 results, and `Fp8` results of up to 32 rows, where it costs nothing, are
+always made so.
+
 On a CUDA tensor every function is a HIP kernel on the current stream of the tensor's device (captured like any other launch) and raises what it does
 not take; on a CPU tensor the same expression runs in PyTorch.  Results have no gradient: inference only, like the 16-bit towers."""
 from __future__ import annotations
@@ -40,7 +46,7 @@ class _GemmArgs(C.Structure):
     """ctypes mirror of `d3d_fp8_gemm_args` (include/dynam3d_hip.h)."""
     _fields_ = ([(n, C.c_void_p) for n in ("x", "sx", "w", "sw", "bias", "residual", "out", "out_scale", "workspace")]
                 + [(n, C.c_int64) for n in ("workspace_bytes", "ldx", "ldsx", "ldw", "ldsw", "ldr", "ldo", "ldos")]
-                + [(n, C.c_int32) for n in ("M", "N", "K", "scale_kind", "out_type", "swiglu")] + [("stream", C.c_void_p)])
+                + [(n, C.c_int32) for n in ("M", "N", "K", "scale_kind", "out_type", "swiglu")] + [("stream", C.c_void_p), ("exact", C.c_int32)])
 
 
 class Fp8:
@@ -252,7 +258,7 @@ def workspace_bytes(m: int, n: int, k: int, swiglu: bool = False, out_dtype: tor
     return _workspace_bytes(m, n, k, int(swiglu), _DT[out_dtype], _KIND[scale_dtype])
 
 
-def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):
+def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu, exact):
     m, k = x.data.shape
     n = w.data.shape[0]
     xd, wd, sx, sw = _rows16(x.data), _rows16(w.data), _unit_rows(x.scale), _unit_rows(w.scale)
@@ -274,7 +280,7 @@ def _gemm(name, x: Fp8, w: Fp8, bias, residual, out_dtype, swiglu):
         residual = _unit_rows(residual)
         rp, ldr = residual.data_ptr(), residual.stride(0)
     a = _GemmArgs(xd.data_ptr(), sx.data_ptr(), wd.data_ptr(), sw.data_ptr(), bp, rp, out.data_ptr(), osp, ws.data_ptr() if nbytes else None, nbytes,
-                  xd.stride(0), sx.stride(0), wd.stride(0), sw.stride(0), ldr, cols, ldos, m, n, k, _KIND[sx.dtype], _DT[out_dtype], swiglu, _stream())
+                  xd.stride(0), sx.stride(0), wd.stride(0), sw.stride(0), ldr, cols, ldos, m, n, k, _KIND[sx.dtype], _DT[out_dtype], swiglu, _stream(), exact)
     _lib.check(_lib.load().d3d_fp8_gemm(C.byref(a)))
     return out if out_scale is None else Fp8._of(out, out_scale)
 
@@ -292,9 +298,10 @@ def _check_operands(name, x, w):
 
 
 def linear(x: Fp8, w: Fp8, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-           out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+           out_dtype: torch.dtype = torch.bfloat16, exact: bool = False) -> torch.Tensor:
     """x w^T [+ bias] [+ residual]: x (M, K), w (N, K), float32 sums, rounded once to `out_dtype` (bf16, fp16, float32 -- the type of bias (N,) and
-    residual (M, N) too).  Any M and N, one row included; K a multiple of 16."""
+    residual (M, N) too).  Any M and N, one row included; K a multiple of 16.  A 16-bit result comes from the 8-bit matrix instruction (see the
+    module), a float32 one, or any with `exact`, from exact products."""
     _check_operands("linear", x, w)
     m, n = x.data.shape[0], w.data.shape[0]
     if out_dtype not in _DT or out_dtype == E4M3:
@@ -312,13 +319,14 @@ def linear(x: Fp8, w: Fp8, bias: Optional[torch.Tensor] = None, residual: Option
             return y.to(out_dtype)
     if x.data.get_device() != _current_device():
         with torch.cuda.device(x.device):
-            return _gemm("linear", x, w, bias, residual, out_dtype, 0)
-    return _gemm("linear", x, w, bias, residual, out_dtype, 0)
+            return _gemm("linear", x, w, bias, residual, out_dtype, 0, bool(exact))
+    return _gemm("linear", x, w, bias, residual, out_dtype, 0, bool(exact))
 
 
-def linear_swiglu(x: Fp8, w: Fp8, out_dtype: torch.dtype = torch.bfloat16):
-    """up * silu(gate) of x w^T, w = [gate (I rows); up (I rows)] as HF's `gate_up_proj` has them, I a multiple of 16; float32 up to the ONE rounding:
-    to bf16 / fp16 / float32, or with out_dtype=torch.float8_e4m3fn to an `Fp8` (scales of the operands' type) for the product that follows."""
+def linear_swiglu(x: Fp8, w: Fp8, out_dtype: torch.dtype = torch.bfloat16, exact: bool = False):
+    """up * silu(gate) of x w^T, w = [gate (I rows); up (I rows)] as HF's `gate_up_proj` has them, I a multiple of 16; float32 sums, rounded once:
+    to bf16 / fp16 / float32, or with out_dtype=torch.float8_e4m3fn to an `Fp8` (scales of the operands' type) for the product that follows.  A float32
+    result, an `Fp8` of up to 32 rows, or any with `exact`, comes from exact products, the others from the 8-bit matrix instruction (see the module)."""
     _check_operands("linear_swiglu", x, w)
     n = w.data.shape[0]
     if out_dtype not in _DT:
@@ -331,5 +339,5 @@ def linear_swiglu(x: Fp8, w: Fp8, out_dtype: torch.dtype = torch.bfloat16):
         return _cpu_quantize(y, x.scale.dtype, 1) if out_dtype == E4M3 else y.to(out_dtype)
     if x.data.get_device() != _current_device():
         with torch.cuda.device(x.device):
-            return _gemm("linear_swiglu", x, w, None, None, out_dtype, 1)
-    return _gemm("linear_swiglu", x, w, None, None, out_dtype, 1)
+            return _gemm("linear_swiglu", x, w, None, None, out_dtype, 1, bool(exact))
+    return _gemm("linear_swiglu", x, w, None, None, out_dtype, 1, bool(exact))

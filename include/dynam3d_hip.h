@@ -646,15 +646,19 @@ int32_t d3d_fp8_rms_norm(const void* x, const void* residual, const float* w, vo
 /* y = xq wq^T with the scales applied, float32 sums, + bias[n] + residual[m,n], rounded once to out_type (0 bf16, 1 fp16, 2 float32; bias and
  * residual have that type; residual may be out).  swiglu: w = [gate (N/2 rows); up (N/2 rows)], y = up * silu(gate), (M, N/2), no bias or
  * residual; out_type 3 = E4M3 + out_scale (M, ceil(N/2/128)) of the same scale_kind.  Both scales are of scale_kind, any
- * finite values: they may multiply out of float32's range where the result does not.  `workspace`: d3d_fp8_gemm_workspace() bytes of device
- * memory on 16 bytes, used until the call's work on `stream` has ended (0: none needed).  K < 2^24; rows of x and w less than 2^24 apart; ldr >= 0
- * (0: one row for all); rows of out and out_scale do not overlap. */
+ * finite values: they may multiply out of float32's range where the result does not.
+ * Products: float32 results, E4M3 results of up to 32 rows, and every result with exact != 0, are float32 sums of exact products.  The others come from the
+ * 8-bit matrix instruction, which drops what lies 13 bits below the largest of 8 neighbouring products: the sum is off by at most
+ * 7 * 2^-13 sum |x w| (~2^-14 of a result of random signs), before the result's own rounding.  exact costs 1 to 3 times the time.
+ * `workspace`: d3d_fp8_gemm_workspace() bytes of device memory on 16 bytes, used until the call's work on `stream` has ended (0: none needed).
+ * K < 2^24; rows of x and w less than 2^24 apart; ldr >= 0 (0: one row for all); rows of out and out_scale do not overlap. */
 typedef struct d3d_fp8_gemm_args {
     const void *x, *sx, *w, *sw, *bias, *residual;
     void *out, *out_scale, *workspace;
     int64_t workspace_bytes, ldx, ldsx, ldw, ldsw, ldr, ldo, ldos;
     int32_t M, N, K, scale_kind, out_type, swiglu;
     void* stream;
+    int32_t exact;
 } d3d_fp8_gemm_args;
 int64_t d3d_fp8_gemm_workspace(int32_t M, int32_t N, int32_t K, int32_t swiglu, int32_t out_type, int32_t scale_kind);
 int32_t d3d_fp8_gemm(const d3d_fp8_gemm_args* a);

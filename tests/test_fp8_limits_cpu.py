@@ -62,3 +62,14 @@ def test_strides_that_the_epilogues_do_not_take():
     for kw in (dict(ldo=-64), dict(ldo=63), dict(ldo=0), dict(ldr=-64, residual=P), dict(large, ldr=-8192), dict(large, ldo=-8192), dict(large, ldo=8184),
                dict(swiglu=1, out_type=3, ldo=16), dict(swiglu=1, N=512, out_type=3, ldo=256, ldos=1), dict(swiglu=1, N=512, out_type=3, ldo=256, ldos=-2)):
         assert refused(b"rows", **kw), (kw, _lib.load().d3d_last_error())
+
+
+def test_workspaces_that_are_too_small_missing_or_off_16_bytes():
+    lib = _lib.load()
+    lds = dict(ldx=4096, ldw=4096, ldsx=32, ldsw=32, K=4096)
+    for kw, need in ((dict(lds, M=100), 100 * 64 * 4 * 8), (dict(lds, M=100, out_type=2), 100 * 64 * 4 * 8), (dict(lds, M=100, scale_kind=1), 100 * 64 * 4 * 8),
+                     (dict(lds, M=4, swiglu=1, out_type=3, ldo=32), 4 * 64 * 4)):
+        assert F8._workspace_bytes(kw["M"], 64, 4096, kw.get("swiglu", 0), kw.get("out_type", 0), kw.get("scale_kind", 0)) == need, kw
+        for bad in (dict(workspace_bytes=need - 1), dict(workspace_bytes=0), dict(workspace=None), dict(workspace=P + 8)):
+            assert refused(b"d3d_fp8_gemm: workspace", **kw, **bad), (kw, bad, lib.d3d_last_error())
+    assert F8.workspace_bytes(4, 64, 4096) == 0 and F8.workspace_bytes(100, 64, 4096) == 100 * 64 * 4 * 8

@@ -96,7 +96,7 @@ __device__ __forceinline__ void dma_piece(uint32_t voff, const void* base, uint3
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_mov_b32 m0, %2\n\t"
-        "s_nop 0\n\t"
+        "s_nop 2\n\t"                                              // 5 wait states in front of the load: its base may come out of a v_readlane (a spilled register)
         "global_load_lds_dwordx4 %1, %3\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(keep)

@@ -47,10 +47,12 @@ __device__ uint4 g_zero16;           // what the lanes behind the end of a ragge
 
 // One 1 KiB piece (8 rows x 128 B) of an operand tile into LDS, 16 bytes per lane, no registers in between.  In asm so that the compiler does
 // not drain it in front of every LDS read (it counts the builtin as a pending LDS write); the K loops wait for it explicitly.
+// The wait states are the assembly's own business too: 1 behind a write of m0, 5 between a vector instruction that writes the scalar base (a v_readlane, where the base
+// was spilled) and the load -- the instructions and the s_nop in front of it make 5 whatever the compiler puts before.
 __device__ __forceinline__ void dma_piece(uint32_t voff, const uint8_t* base, uint32_t dst) {
     const uint32_t d = __builtin_amdgcn_readfirstlane(dst);
     uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
 }
 __device__ __forceinline__ void dma_piece_at(const uint8_t* addr, uint32_t dst) {
@@ -62,7 +64,7 @@ __device__ __forceinline__ void dma_piece_at(const uint8_t* addr, uint32_t dst) 
 __device__ __forceinline__ void dma_piece_once(uint32_t voff, const uint8_t* base, uint32_t dst) {      // data read once: not kept in the caches
     const uint32_t d = __builtin_amdgcn_readfirstlane(dst);
     uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
 }
 // one scale per lane (a byte, or a float32) into the dwords behind LDS dst
@@ -71,10 +73,10 @@ __device__ __forceinline__ void dma_scale(uint32_t voff, const uint8_t* base, ui
     const uint32_t d = __builtin_amdgcn_readfirstlane(dst);
     uint32_t keep;
     if constexpr (KIND == 0)
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %3\n\ts_mov_b32 m0, %0"
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 2\n\tglobal_load_lds_ubyte %1, %3\n\ts_mov_b32 m0, %0"
                      : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
     else
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 2\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
                      : "=&s"(keep) : "v"(voff), "s"(d), "s"(base) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
@@ -545,7 +547,8 @@ k_fp8_gemm_tile(const GemmArgs a) {
 // DT: 0 bf16, 1 fp16, 3 E4M3 + scale (SwiGLU).  Rows of out and residual allow 16-byte accesses, columns come in eights (the host's choice of this kernel).
 // ================================================================================================================================
 // 1 KiB (16 bytes per lane from base + off), or one byte per lane into a dword, to LDS dst + IMM; base and dst in scalar registers.  (m0 is not kept: nothing else
-// in the kernel below uses it.)
+// in the kernel below uses it.  2 wait states of its own: the bases are made, by v_readfirstlane, a dozen products or an s_nop 4 ahead -- and none is spilled.  With 5 here, 18
+// times per K tile, 6568 x 9216 x 3072 took 163.5 us instead of 160.)
 template <int IMM>
 __device__ __forceinline__ void dma_to(uint32_t off, const uint8_t* base, uint32_t dst) {
     asm volatile("s_add_u32 m0, %1, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(off), "s"(dst), "s"(base), "n"(IMM) : "memory", "scc");
@@ -674,6 +677,9 @@ k_fp8_gemm_big(const GemmArgs a) {
 
     // nk >= 2 (the host's choice of this kernel)
     const From f0 = from(0, 0), f1 = from(1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 4" ::: "memory");                              // the bases have reached the scalar registers
+    __builtin_amdgcn_sched_barrier(0);
     if (ragged) {                                                      // the chunks behind K read zeros
         const bool in = (nk - 1) * FP8_G + chunk * 16 < a.K;
 #pragma unroll

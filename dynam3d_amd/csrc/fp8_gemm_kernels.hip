@@ -541,7 +541,7 @@ k_fp8_gemm_tile(const GemmArgs a) {
 //   * Rows are permuted inside blocks of 64: row 4 f + c of a block is row f of tile c, for x and w alike.  A lane then holds 16 NEIGHBOURING columns of a row
 //     (it stores them with no trip through LDS), and the scales of its rows in four tiles are neighbours: they come by DMA too, a dword per row, are
 //     read as one 16-byte piece, and packed into a register of which the instruction picks the byte.
-//   * What bounds it: power, then waits.  8192^3 402 - 440 us, 2.5 - 2.7 PFLOP/s; the matrix pipe is busy 70 % of the cycles, at 1.8 GHz; 16 % are waits for loads and at
+//   * What bounds it: power, then waits.  8192^3 402 - 440 us, 2.5 - 2.7 PFLOP/s; the matrix pipe is busy 70 % of the cycles there, at 1.8 GHz (6568 x 9216 x 3072, 24 K tiles and a round of 168 tiles at the end: 53 %); 16 % are waits for loads and at
 //     the barriers; with a quarter of the CUs at work a K tile takes 0.97 us instead of 1.7.  One workgroup
 //     for several output tiles, loading the next one's operands while it stores, gained nothing (172.7 and 171.8 us for 6568 x 9216 x 3072).
 // DT: 0 bf16, 1 fp16, 3 E4M3 + scale (SwiGLU).  Rows of out and residual allow 16-byte accesses, columns come in eights (the host's choice of this kernel).

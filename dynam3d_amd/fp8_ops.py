@@ -301,7 +301,8 @@ def linear(x: Fp8, w: Fp8, bias: Optional[torch.Tensor] = None, residual: Option
            out_dtype: torch.dtype = torch.bfloat16, exact: bool = False) -> torch.Tensor:
     """x w^T [+ bias] [+ residual]: x (M, K), w (N, K), float32 sums, rounded once to `out_dtype` (bf16, fp16, float32 -- the type of bias (N,) and
     residual (M, N) too).  Any M and N, one row included; K a multiple of 16.  A 16-bit result comes from the 8-bit matrix instruction (see the
-    module), a float32 one, or any with `exact`, from exact products."""
+    module), a float32 one, or any with `exact`, from exact products.  Large products are fastest with N a multiple of 8 and residual rows that start on
+    16 bytes (6568 x 9216 x 3072: 194 us, 395 where they do not)."""
     _check_operands("linear", x, w)
     m, n = x.data.shape[0], w.data.shape[0]
     if out_dtype not in _DT or out_dtype == E4M3:

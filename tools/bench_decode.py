@@ -1,6 +1,6 @@
 """Decode-only latency of the Phi-3 stack (8 sequences, KV cache): ms per generated token = (T tokens - 2 tokens) / (T - 2) on the same prefill,
 min over repetitions, for the launch-per-op path with 1 / 2 / 4 / 8 key ranges in the decode attention and for the persistent kernel.
-usage: bench_decode.py [prompt_len=864] [layers=32]"""
+usage: bench_decode.py [prompt_len=864] [layers=32] [fp8] [sequences=8]      (fp8: Phi3Decoder(quant="fp8"), its one path; prints the prefill too)"""
 import os
 import sys
 
@@ -13,13 +13,16 @@ from dynam3d_amd.weights import synth_state_dict
 
 S = int(sys.argv[1]) if len(sys.argv) > 1 else 864
 layers = int(sys.argv[2]) if len(sys.argv) > 2 else 32
+quant = "fp8" if "fp8" in sys.argv[3:] else None
+B = int(sys.argv[-1]) if len(sys.argv) > 3 and sys.argv[-1].isdigit() else 8
 D.enable_hip_kernels(["all"])
 cfg = Phi3Config(vocab=32064, hidden=3072, layers=layers, heads=32, kv_heads=32, mlp=8192)
 sd = synth_state_dict(phi3_param_spec(cfg), seed=3, device="cuda", dtype_for=lambda n: torch.float32 if "norm" in n else torch.bfloat16)
-dec = Phi3Decoder(sd, cfg, torch.bfloat16, "cuda")
+dec = Phi3Decoder(sd, cfg, torch.bfloat16, "cuda", quant=quant)
 del sd
-lens = [S] * 8
-x = (torch.randn(sum(lens), cfg.hidden, device="cuda") * 0.5).to(torch.bfloat16)
+lens = [S] * B
+x = torch.zeros(((sum(lens) + 255) // 256 * 256, cfg.hidden), device="cuda", dtype=torch.bfloat16)
+x[:sum(lens)] = torch.randn(sum(lens), cfg.hidden, device="cuda") * 0.5
 T = 34
 
 
@@ -33,8 +36,8 @@ def timed(n):
     return a.elapsed_time(b)
 
 
-weights_gb = layers * (9216 * 3072 + 3072 * 3072 + 16384 * 3072 + 3072 * 8192) * 2 / 1e9 + 32064 * 3072 * 2 / 1e9
-kv_gb = layers * 8 * S * 2 * 3072 * 2 / 1e9
+weights_gb = layers * (9216 * 3072 + 3072 * 3072 + 16384 * 3072 + 3072 * 8192) * (1 if quant else 2) / 1e9 + 32064 * 3072 * 2 / 1e9
+kv_gb = layers * B * S * 2 * 3072 * 2 / 1e9
 modes = [("launch-per-op, 1 key range", {"D3D_DECODE_PERSISTENT": "0", "D3D_DECODE_SPLIT": "1"}),
          ("launch-per-op, 2 key ranges", {"D3D_DECODE_PERSISTENT": "0", "D3D_DECODE_SPLIT": "2"}),
          ("launch-per-op, 4 key ranges", {"D3D_DECODE_PERSISTENT": "0", "D3D_DECODE_SPLIT": "4"}),
@@ -53,6 +56,18 @@ if os.environ.get("BENCH_DECODE_R05") == "1":        # round 5: one-pass decode 
 if os.environ.get("BENCH_DECODE_R05") == "2":        # one-pass attention: waves per workgroup x keys in flight
     base = {"D3D_DECODE_PERSISTENT": "0", "D3D_DECODE_SPLIT": "1", "D3D_DECODE_ATTN": "2", "D3D_SKINNY_NT": "0"}
     modes = [(f"one-pass attention, cfg {c}", dict(base, D3D_DECODE_ATTN2_CFG=c)) for _ in range(2) for c in ("804", "404", "1604", "808", "1608")]
+if quant or len(sys.argv) > 3:
+    modes = [("8-bit linears" if quant else "16-bit linears, default", {})] * 2
+
+    def prefill():
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        dec.prefill_logits_packed(x, lens)
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b)
+    prefill(), prefill()
+    print(f"prefill of {B} x {S} tokens: {min(prefill() for _ in range(10)):.2f} ms (least of 10)", flush=True)
 for name, env in modes:
     os.environ.pop("D3D_DECODE_SPLIT", None)
     os.environ.update(env)

@@ -256,7 +256,9 @@ class LlavaVisionTower(_VitTrunk):
 class Phi3Decoder:
     """`quant`: None -- weights and activations in `dtype` -- or "fp8": the four linears of every layer on E4M3 operands (`fp8_ops`: weights with one
     power-of-two scale per 128 x 128 block, quantised once at load; activations with one per row and 128 columns, quantised where they are made: by the
-    RMSNorm, behind the attention, by the SwiGLU product).  The residual stream, the attention with its KV cache, the embedding and lm_head stay in `dtype`."""
+    RMSNorm, behind the attention, by the SwiGLU product).  The residual stream, the attention with its KV cache, the embedding and lm_head stay in `dtype`.
+    The products are `fp8_ops`' default ones: of a prompt's rows on the 8-bit matrix instruction, of up to 32 rows with an exact SwiGLU product (exact prompts would
+    take longer than 16-bit ones)."""
 
     def __init__(self, sd: Dict[str, torch.Tensor], cfg: Phi3Config = Phi3Config(), dtype=torch.bfloat16, device="cuda", quant: Optional[str] = None):
         if quant not in (None, "fp8"):
